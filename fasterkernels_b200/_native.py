@@ -17,9 +17,11 @@ from .build import LIB_PATH
 FK_DTYPE_F16 = 0
 FK_DTYPE_BF16 = 1
 FK_DTYPE_E4M3 = 2
+FK_DTYPE_F32 = 3  # cos / sin tables and norm weights only
 
 FK_STATUS_BAD_PAGE = 1
 FK_STATUS_TIMEOUT = 2
+FK_STATUS_BAD_POSITION = 4
 
 _DTYPE_CODES = {
     torch.float16: FK_DTYPE_F16,
@@ -87,6 +89,8 @@ def lib() -> ctypes.CDLL:
             _I, _I, _I, _L, _I,                  # batch kv_heads head_dim num_pages max_blocks
             _L, _L, _L, _L, _L, _L, _L, _L, _L, _L, _L,
             _P]
+        L.fk_qk_norm_rope.restype = _I
+        L.fk_qk_norm_rope.argtypes = [ctypes.c_char_p, _P]  # packed fk_rope_args, stream
         L.fk_profile_begin.restype = _I
         L.fk_profile_begin.argtypes = [_I]
         L.fk_profile_end.restype = _I

@@ -14,6 +14,7 @@ bit-identical.
 """
 from __future__ import annotations
 
+import struct
 from typing import Optional
 
 import torch
@@ -90,6 +91,62 @@ def append_launch(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor
     N.check(rc, "fk_paged_kv_append")
 
 
+_ROPE_ARGS = struct.Struct("17Q34qd")  # fk_rope_args of include/fk_decode.h
+_WIDE_CODES = {torch.float16: N.FK_DTYPE_F16, torch.bfloat16: N.FK_DTYPE_BF16, torch.float32: N.FK_DTYPE_F32}
+
+
+def _addr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _rows16(t):
+    """t, or a copy whose rows start on 16-byte boundaries (an unaligned or
+    inner-strided view)."""
+    e = t.element_size()
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s * e % 16 == 0 for s in t.stride()[:-1]):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def rope_launch(q: torch.Tensor, k: torch.Tensor, v: Optional[torch.Tensor], cos: Optional[torch.Tensor],
+                sin: Optional[torch.Tensor], positions: Optional[torch.Tensor], seq_ids: Optional[torch.Tensor],
+                bt: Optional[torch.Tensor], q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
+                eps: float, interleaved: bool, scale_k: Optional[torch.Tensor], scale_v: Optional[torch.Tensor],
+                q_out: torch.Tensor, k_out: Optional[torch.Tensor], k_pool: Optional[torch.Tensor],
+                v_pool: Optional[torch.Tensor], status: Optional[torch.Tensor]) -> None:
+    T, QH, D = q.shape
+    if T == 0:
+        return
+    q, k = _rows16(q), _rows16(k)
+    R = max_pos = cos_row = sin_row = table = 0
+    if cos is not None:
+        cos, sin = _rows16(cos), _rows16(sin)
+        R, max_pos, table = 2 * cos.shape[1], cos.shape[0], _WIDE_CODES[cos.dtype]
+        cos_row, sin_row = cos.stride(0), sin.stride(0)
+    if q_weight is not None:
+        q_weight = _rows16(q_weight)
+    if k_weight is not None:
+        k_weight = _rows16(k_weight)
+    qs, ks, qos = q.stride(), k.stride(), q_out.stride()
+    kos = (0, 0) if k_out is None else k_out.stride()
+    vs, kps, vps, pool_code, bt_b, bt_rows, blocks, pages = (0, 0), (0, 0, 0), (0, 0, 0), 0, 0, 0, 0, 0
+    if k_pool is not None:
+        v = _rows16(v)
+        vs, kps, vps = v.stride(), k_pool.stride(), v_pool.stride()
+        pool_code, pages = N.dtype_code(k_pool.dtype), k_pool.shape[0]
+        bt_b, bt_rows, blocks = bt.stride(0), bt.shape[0], bt.shape[1]
+    args = _ROPE_ARGS.pack(
+        q.data_ptr(), k.data_ptr(), _addr(v), q_out.data_ptr(), _addr(k_out), _addr(k_pool), _addr(v_pool), _addr(cos),
+        _addr(sin), _addr(positions), _addr(seq_ids), _addr(bt), _addr(q_weight), _addr(k_weight), _addr(scale_k),
+        _addr(scale_v), _addr(status),
+        qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], qos[0], qos[1], kos[0], kos[1],
+        kps[0], kps[1], kps[2], vps[0], vps[1], vps[2], cos_row, sin_row, bt_b,
+        T, QH, k.shape[1], D, R, interleaved, max_pos, bt_rows, blocks, pages, N.dtype_code(q.dtype), pool_code, table,
+        0 if q_weight is None else _WIDE_CODES[q_weight.dtype], 0 if k_weight is None else _WIDE_CODES[k_weight.dtype],
+        eps)
+    N.check(N.lib().fk_qk_norm_rope(args, N.stream_of(q.device)), "fk_qk_norm_rope")
+
+
 # ---------------------------------------------------------------- custom ops
 _LIB = "fasterkernels_b200"
 
@@ -122,9 +179,21 @@ def _append_op(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor, v
     append_launch(k_new, v_new, k_pool, v_pool, bt, positions, increment, scale_k, scale_v, status)
 
 
+@torch.library.custom_op(f"{_LIB}::qk_norm_rope", mutates_args=("q_out", "k_out", "k_pool", "v_pool", "status"),
+                         device_types="cuda")
+def _rope_op(q: torch.Tensor, k: torch.Tensor, v: Optional[torch.Tensor], cos: Optional[torch.Tensor],
+             sin: Optional[torch.Tensor], positions: Optional[torch.Tensor], seq_ids: Optional[torch.Tensor],
+             bt: Optional[torch.Tensor], q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
+             eps: float, interleaved: bool, scale_k: Optional[torch.Tensor], scale_v: Optional[torch.Tensor],
+             q_out: torch.Tensor, k_out: Optional[torch.Tensor], k_pool: Optional[torch.Tensor],
+             v_pool: Optional[torch.Tensor], status: Optional[torch.Tensor]) -> None:
+    rope_launch(q, k, v, cos, sin, positions, seq_ids, bt, q_weight, k_weight, eps, interleaved, scale_k, scale_v,
+                q_out, k_out, k_pool, v_pool, status)
+
+
 # The outputs are preallocated by the callers, so the fake (meta)
 # implementations have nothing to compute.
-for _op in (_varlen_op, _dense_op, _paged_op, _append_op):
+for _op in (_varlen_op, _dense_op, _paged_op, _append_op, _rope_op):
     _op.register_fake(lambda *args, **kwargs: None)
 
 
@@ -140,3 +209,4 @@ varlen = _dispatch(_varlen_op, varlen_launch)
 dense = _dispatch(_dense_op, dense_launch)
 paged = _dispatch(_paged_op, paged_launch)
 append = _dispatch(_append_op, append_launch)
+rope = _dispatch(_rope_op, rope_launch)

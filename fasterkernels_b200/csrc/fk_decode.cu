@@ -15,6 +15,7 @@
 #include <string>
 
 #include "fk_decode_kernel.cuh"
+#include "fk_host.h"
 
 // The kernels are instantiated in fk_kernels_{f16,bf16,e4m3}.cu; a build of
 // this file alone (e.g. the -DFK_TRACE diagnostics build) defines
@@ -254,12 +255,22 @@ std::atomic<int> g_inject{0};
 // the decode grid may be scheduled while the previous kernel of its stream
 // drains, and executes griddepcontrol.wait before its first global read, so
 // whatever that kernel wrote (KV append, RoPE'd Q, new lengths) is visible.
-inline bool pdl_enabled() {
+bool pdl_enabled() {
   static const bool on = [] {
     const char* e = getenv("FK_DECODE_PDL");
     return !(e != nullptr && e[0] == '0');
   }();
   return on;
+}
+
+int pointer_device(const void* p, const char* name, int* device) {
+  cudaPointerAttributes attr;
+  if (cudaPointerGetAttributes(&attr, p) != cudaSuccess || attr.type != cudaMemoryTypeDevice) {
+    cudaGetLastError();
+    return fail(FK_ERR_INVALID_ARG, "%s must be device memory", name);
+  }
+  *device = attr.device;
+  return FK_OK;
 }
 
 template <int KV, int LAYOUT, int HP, int D, bool CP, bool QC>

@@ -46,6 +46,7 @@ extern "C" {
 #define FK_DTYPE_F16 0
 #define FK_DTYPE_BF16 1
 #define FK_DTYPE_E4M3 2 /* float8_e4m3fn */
+#define FK_DTYPE_F32 3  /* cos / sin tables and norm weights only */
 
 /* return codes */
 #define FK_OK 0
@@ -58,6 +59,7 @@ extern "C" {
 /* bits of the device status word (first int32 of the workspace) */
 #define FK_STATUS_BAD_PAGE 1 /* block-table entry outside [0, num_pages): page skipped, its tokens masked */
 #define FK_STATUS_TIMEOUT 2  /* a pipeline wait ran past its bound and the CTA gave up */
+#define FK_STATUS_BAD_POSITION 4 /* a token's position is negative or past the cos / sin tables */
 
 /* Library version, e.g. 100 for 0.1.0. */
 int fk_version(void);
@@ -183,6 +185,63 @@ int fk_paged_kv_append(const void* k_new, const void* v_new, int in_dtype, void*
                        int head_dim, int64_t num_pages, int max_blocks, int64_t skn_b, int64_t skn_h,
                        int64_t svn_b, int64_t svn_h, int64_t sk_p, int64_t sk_h, int64_t sk_s,
                        int64_t sv_p, int64_t sv_h, int64_t sv_s, int64_t bt_b, void* stream);
+
+/*
+ * Per-head RMS norm and position rotation of queries and keys in one pass,
+ * and the same on the way into a paged KV cache (no counterpart in the
+ * reference: its models normalise, rotate and append in separate torch ops).
+ * For token t and each head row x[D] of q and k, computed in 32 bits and
+ * rounded once to the output's type:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight     when the weight is non-null
+ *   (a, b) -> (a cos - b sin, b cos + a sin)    for the rotary_dim / 2 pairs
+ *       of the first rotary_dim dims: dims (i, i + rotary_dim / 2), or
+ *       (2i, 2i + 1) when `interleaved`; cos / sin row positions[t].
+ * q_out gets the rows of q; k_out (when non-null) those of k.  With k_pool
+ * non-null, the rows of k and of v (v as it is) are also written to page
+ * block_table[seq, pos / 16], slot pos % 16, of sequence seq = seq_ids[t] (t
+ * itself when seq_ids is null); e4m3 pools store e4m3(clamp(x / scale, +-448)).
+ *
+ * Device-side conditions set a bit of *status (when non-null): a position
+ * that is negative or past the tables (FK_STATUS_BAD_POSITION: the token's
+ * q_out / k_out rows are zeroed, nothing is appended); a sequence outside
+ * [0, table_rows), a page past max_blocks or an entry outside [0, num_pages)
+ * (FK_STATUS_BAD_PAGE: nothing is appended).  No two tokens of a call may share
+ * a slot.  q_out / k_out may be q / k themselves (same strides); other overlap
+ * is not allowed.  positions may be null without a pool: token t then takes
+ * table row t % max_pos.
+ *
+ * Every field is 8 bytes; strides are in elements, inner strides 1; rows,
+ * strides, tables and weights are 16-byte aligned.  rotary_dim is a multiple of
+ * 16 (0: no rotation, cos / sin unused); head_dim 128 or 64.
+ */
+typedef struct fk_rope_args {
+  const void* q;       /* [tokens, q_heads, D] f16/bf16 */
+  const void* k;       /* [tokens, kv_heads, D] */
+  const void* v;       /* [tokens, kv_heads, D], with a pool */
+  void* q_out;
+  void* k_out;
+  void* k_pool;        /* [num_pages, kv_heads, 16, D], dtype or E4M3; null: no append */
+  void* v_pool;
+  const void* cos;     /* [max_pos, rotary_dim / 2] */
+  const void* sin;
+  const void* positions;    /* int32 [tokens] */
+  const void* seq_ids;      /* int32 [tokens] or null */
+  const void* block_table;  /* int32 [table_rows, max_blocks] */
+  const void* q_weight;     /* [D] or null */
+  const void* k_weight;
+  const void* scale_k;      /* float, e4m3 pools */
+  const void* scale_v;
+  void* status;             /* int32 or null */
+  int64_t q_t, q_h, k_t, k_h, v_t, v_h, qo_t, qo_h, ko_t, ko_h;
+  int64_t kp_p, kp_h, kp_s, vp_p, vp_h, vp_s;
+  int64_t cos_row, sin_row, bt_b;
+  int64_t tokens, q_heads, kv_heads, head_dim, rotary_dim, interleaved, max_pos;
+  int64_t table_rows, max_blocks, num_pages;
+  int64_t dtype, pool_dtype, table_dtype, q_weight_dtype, k_weight_dtype;
+  double eps;
+} fk_rope_args;
+
+int fk_qk_norm_rope(const fk_rope_args* args, void* stream);
 
 /*
  * Measurement hooks (no reference counterpart: the reference times with
