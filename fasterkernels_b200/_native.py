@@ -91,6 +91,10 @@ def lib() -> ctypes.CDLL:
             _P]
         L.fk_qk_norm_rope.restype = _I
         L.fk_qk_norm_rope.argtypes = [ctypes.c_char_p, _P]  # packed fk_rope_args, stream
+        L.fk_shared_prefix_workspace_bytes.restype = _Z
+        L.fk_shared_prefix_workspace_bytes.argtypes = [_I, _I, _I, _I, _I, _I]
+        L.fk_paged_shared_prefix_decode.restype = _I
+        L.fk_paged_shared_prefix_decode.argtypes = [ctypes.c_char_p, _P, _Z, _P]  # packed fk_prefix_args
         L.fk_profile_begin.restype = _I
         L.fk_profile_begin.argtypes = [_I]
         L.fk_profile_end.restype = _I
@@ -173,6 +177,27 @@ def workspace(device: torch.device, batch: int, q_heads: int, kv_heads: int, kv_
         return ws
 
 
+_status = {}
+
+
+def status_word(device: torch.device) -> torch.Tensor:
+    """The device's sticky FK_STATUS_* word for operators whose scratch is
+    allocated per call (one int32 that ``read_status`` reads).  Made by the first
+    eager call; a graph captures its address."""
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    w = _status.get(idx)
+    if w is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the status word must exist before CUDA graph capture: run one eager call first")
+        with _ws_lock:
+            w = _status.get(idx)
+            if w is None:
+                w = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+                torch.cuda.synchronize(idx)  # once: visible to every stream
+                _status[idx] = w
+    return w
+
+
 def device_workspaces(device=None):
     """The cached workspaces of a device (one per stream that decoded on it)."""
     idx = torch.cuda.current_device() if device is None else torch.device(device).index
@@ -186,6 +211,12 @@ def read_status(device=None, clear: bool = True) -> int:
     off the hot path.  After FK_STATUS_TIMEOUT the whole workspace is cleared
     when clearing: a kernel that gave up may leave arrival counters mid-count."""
     st = 0
+    idx = torch.cuda.current_device() if device is None else torch.device(device).index
+    word = _status.get(idx)
+    if word is not None:
+        st = int(word.item())
+        if clear:
+            word.zero_()
     for ws in device_workspaces(device):
         w = int(ws[:4].view(torch.int32).item())
         st |= w

@@ -147,6 +147,42 @@ def rope_launch(q: torch.Tensor, k: torch.Tensor, v: Optional[torch.Tensor], cos
     N.check(N.lib().fk_qk_norm_rope(args, N.stream_of(q.device)), "fk_qk_norm_rope")
 
 
+_PREFIX_ARGS = struct.Struct("13Q22q")  # fk_prefix_args of include/fk_decode.h
+_prefix_ws_bytes = {}
+
+
+def shared_prefix_launch(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, prefix_table: torch.Tensor,
+                         prefix_len: Optional[torch.Tensor], prefix_len_host: int, bt: torch.Tensor, lens: torch.Tensor,
+                         s_aux: Optional[torch.Tensor], scale_q: Optional[torch.Tensor],
+                         scale_k: Optional[torch.Tensor], scale_v: Optional[torch.Tensor], out: torch.Tensor) -> None:
+    dev = q.device
+    B, QH, D = q.shape
+    if B == 0:
+        return
+    P, KVH, _, _ = k_pool.shape
+    kv_code = N.dtype_code(k_pool.dtype)
+    lib = N.lib()
+    key = (dev.index, B, QH, KVH, D, kv_code)
+    need = _prefix_ws_bytes.get(key)
+    if need is None:
+        need = int(lib.fk_shared_prefix_workspace_bytes(*key))
+        if need == 0:
+            raise RuntimeError(f"fk_shared_prefix_workspace_bytes failed: {N.last_error()}")
+        _prefix_ws_bytes[key] = need
+    status = N.status_word(dev)
+    # scratch of this call alone (torch's allocator reuses it in stream order;
+    # in a captured graph it belongs to the graph's pool), so calls on other
+    # streams and other graphs never share it
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    qs, ks, vs, os = q.stride(), k_pool.stride(), v_pool.stride(), out.stride()
+    args = _PREFIX_ARGS.pack(
+        q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), prefix_table.data_ptr(), _addr(prefix_len), bt.data_ptr(),
+        lens.data_ptr(), _addr(s_aux), out.data_ptr(), _addr(scale_q), _addr(scale_k), _addr(scale_v), status.data_ptr(),
+        prefix_len_host, prefix_table.shape[0], B, QH, KVH, D, P, bt.shape[1], N.dtype_code(q.dtype), kv_code,
+        N.dtype_code(out.dtype), qs[0], qs[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], bt.stride(0), os[0], os[1])
+    N.check(lib.fk_paged_shared_prefix_decode(args, N.ptr(ws), need, N.stream_of(dev)), "fk_paged_shared_prefix_decode")
+
+
 # ---------------------------------------------------------------- custom ops
 _LIB = "fasterkernels_b200"
 
@@ -191,9 +227,18 @@ def _rope_op(q: torch.Tensor, k: torch.Tensor, v: Optional[torch.Tensor], cos: O
                 q_out, k_out, k_pool, v_pool, status)
 
 
+@torch.library.custom_op(f"{_LIB}::shared_prefix_decode", mutates_args=("out",), device_types="cuda")
+def _shared_prefix_op(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, prefix_table: torch.Tensor,
+                      prefix_len: Optional[torch.Tensor], prefix_len_host: int, bt: torch.Tensor, lens: torch.Tensor,
+                      s_aux: Optional[torch.Tensor], scale_q: Optional[torch.Tensor], scale_k: Optional[torch.Tensor],
+                      scale_v: Optional[torch.Tensor], out: torch.Tensor) -> None:
+    shared_prefix_launch(q, k_pool, v_pool, prefix_table, prefix_len, prefix_len_host, bt, lens, s_aux, scale_q, scale_k,
+                         scale_v, out)
+
+
 # The outputs are preallocated by the callers, so the fake (meta)
 # implementations have nothing to compute.
-for _op in (_varlen_op, _dense_op, _paged_op, _append_op, _rope_op):
+for _op in (_varlen_op, _dense_op, _paged_op, _append_op, _rope_op, _shared_prefix_op):
     _op.register_fake(lambda *args, **kwargs: None)
 
 
@@ -210,3 +255,4 @@ dense = _dispatch(_dense_op, dense_launch)
 paged = _dispatch(_paged_op, paged_launch)
 append = _dispatch(_append_op, append_launch)
 rope = _dispatch(_rope_op, rope_launch)
+shared_prefix = _dispatch(_shared_prefix_op, shared_prefix_launch)

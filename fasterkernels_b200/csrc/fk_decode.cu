@@ -16,6 +16,7 @@
 
 #include "fk_decode_kernel.cuh"
 #include "fk_host.h"
+#include "fk_prefix.h"
 
 // The kernels are instantiated in fk_kernels_{f16,bf16,e4m3}.cu; a build of
 // this file alone (e.g. the -DFK_TRACE diagnostics build) defines
@@ -519,19 +520,20 @@ extern "C" int fk_flash_decode_gqa_hf_dense(const void* q, const void* k_cache, 
   return launch<DENSE>(p, kv_dtype, device, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
-extern "C" int fk_paged_flash_decode(const void* q, const void* k_pool, const void* v_pool,
+namespace fk {
+
+// Argument checks and tensor maps of a paged call, everything short of the
+// launch.  Returns FK_EMPTY for an empty batch.
+int paged_prepare(Params& p, int* device, const void* q, const void* k_pool, const void* v_pool,
                                      const int32_t* block_table, const int32_t* seq_lens, const float* s_aux,
                                      void* out, int batch, int q_heads, int kv_heads, int head_dim,
                                      int64_t num_pages, int page_size, int max_blocks, int q_dtype, int kv_dtype,
                                      int out_dtype, const float* scale_q, const float* scale_k,
                                      const float* scale_v, int64_t sq_b, int64_t sq_h, int64_t sk_p, int64_t sk_h,
                                      int64_t sk_s, int64_t sv_p, int64_t sv_h, int64_t sv_s, int64_t bt_b,
-                                     int64_t so_b, int64_t so_h, void* workspace, size_t workspace_bytes,
-                                     void* stream) {
-  int device = 0;
+                                     int64_t so_b, int64_t so_h, void* workspace) {
   int rc = common_checks(q, k_pool, v_pool, out, batch, q_heads, kv_heads, head_dim, q_dtype, kv_dtype, out_dtype,
-                         workspace, &device);
-  if (rc == FK_EMPTY) return FK_OK;
+                         workspace, device);
   if (rc != FK_OK) return rc;
   if ((rc = check_q_align(q, q_dtype, sq_b, sq_h)) != FK_OK) return rc;
   if (page_size != PAGE) return fail(FK_ERR_UNSUPPORTED, "page_size must be 16 (got %d)", page_size);
@@ -543,7 +545,6 @@ extern "C" int fk_paged_flash_decode(const void* q, const void* k_pool, const vo
   if (((sk_p | sk_h | sk_s | sv_p | sv_h | sv_s) * es) % 16 != 0)
     return fail(FK_ERR_INVALID_ARG, "k/v pool strides must be multiples of 16 bytes");
   if (num_pages > 0x7fffffffLL) return fail(FK_ERR_INVALID_ARG, "num_pages too large");
-  Params p;
   memset(&p, 0, sizeof(p));
   fill_common(p, q, sq_b, sq_h, out, so_b, so_h, s_aux, batch, q_heads, kv_heads, head_dim, q_dtype, out_dtype, scale_q,
               scale_k, scale_v, workspace);
@@ -576,6 +577,60 @@ extern "C" int fk_paged_flash_decode(const void* q, const void* k_pool, const vo
     if ((rc = encode_map(&p.tk, kv_dtype, 5, k_pool, dims, ks, box)) != FK_OK) return rc;
     if ((rc = encode_map(&p.tv, kv_dtype, 5, v_pool, dims, vs, box)) != FK_OK) return rc;
   }
+  return FK_OK;
+}
+
+int own_part_prepare(OwnPart* own, const fk_prefix_args& a, void* workspace, int* device) {
+  // a batch whose own tables have no columns still gets its (empty) part
+  const void* bt = (a.max_blocks == 0 && a.block_table == nullptr) ? a.seq_lens : a.block_table;
+  const int rc = paged_prepare(own->p, device, a.q, a.k_pool, a.v_pool, static_cast<const int32_t*>(bt),
+                               static_cast<const int32_t*>(a.seq_lens), nullptr, a.out, static_cast<int>(a.batch),
+                               static_cast<int>(a.q_heads), static_cast<int>(a.kv_heads), static_cast<int>(a.head_dim),
+                               a.num_pages, PAGE, static_cast<int>(a.max_blocks), static_cast<int>(a.q_dtype),
+                               static_cast<int>(a.kv_dtype), static_cast<int>(a.out_dtype),
+                               static_cast<const float*>(a.scale_q), static_cast<const float*>(a.scale_k),
+                               static_cast<const float*>(a.scale_v), a.q_b, a.q_h, a.kp_p, a.kp_h, a.kp_s, a.vp_p, a.vp_h,
+                               a.vp_s, a.bt_b, a.o_b, a.o_h, workspace);
+  if (rc != FK_OK) return rc;
+  own->kv = static_cast<int>(a.kv_dtype);
+  own->device = *device;
+  own->q_al16 = own->p.q_al16;
+  return FK_OK;
+}
+
+int own_part_zero_words(const OwnPart&, size_t ws_bytes) {
+  return static_cast<int>(64 + (ws_bytes > 256 ? (ws_bytes - 256) / SEG_BYTES : 0));  // header + counters (WsLayout)
+}
+
+int own_part_launch(OwnPart& own, float2* ml, float* acc, size_t ws_bytes, cudaStream_t stream) {
+  own.p.part_ml = ml;
+  own.p.part_acc = acc;
+  return launch<PAGED>(own.p, own.kv, own.device, ws_bytes, stream);
+}
+
+void debug_settings(unsigned long long* wait_ns, int* inject) {
+  *wait_ns = g_wait_ns.load();
+  *inject = g_inject.load();
+}
+
+}  // namespace fk
+
+extern "C" int fk_paged_flash_decode(const void* q, const void* k_pool, const void* v_pool,
+                                     const int32_t* block_table, const int32_t* seq_lens, const float* s_aux,
+                                     void* out, int batch, int q_heads, int kv_heads, int head_dim,
+                                     int64_t num_pages, int page_size, int max_blocks, int q_dtype, int kv_dtype,
+                                     int out_dtype, const float* scale_q, const float* scale_k,
+                                     const float* scale_v, int64_t sq_b, int64_t sq_h, int64_t sk_p, int64_t sk_h,
+                                     int64_t sk_s, int64_t sv_p, int64_t sv_h, int64_t sv_s, int64_t bt_b,
+                                     int64_t so_b, int64_t so_h, void* workspace, size_t workspace_bytes,
+                                     void* stream) {
+  int device = 0;
+  Params p;
+  const int rc = paged_prepare(p, &device, q, k_pool, v_pool, block_table, seq_lens, s_aux, out, batch, q_heads, kv_heads,
+                               head_dim, num_pages, page_size, max_blocks, q_dtype, kv_dtype, out_dtype, scale_q, scale_k,
+                               scale_v, sq_b, sq_h, sk_p, sk_h, sk_s, sv_p, sv_h, sv_s, bt_b, so_b, so_h, workspace);
+  if (rc == FK_EMPTY) return FK_OK;
+  if (rc != FK_OK) return rc;
   return launch<PAGED>(p, kv_dtype, device, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 

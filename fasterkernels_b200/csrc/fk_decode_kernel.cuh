@@ -199,6 +199,11 @@ struct Params {
   int o_al8;   // out base and strides 8-byte aligned (four outputs per store)
   int qc;      // query chunks of at most 8 heads per KV head: ceil(G / 8)
   int head_dim;  // D (the kernel is instantiated per D; kept for host checks)
+  // Own part of a shared-prefix decode: when set, the running (max, sum) and
+  // accumulators of each (sequence, query head) are stored here instead of
+  // being normalised into `out`.
+  float2* part_ml;
+  float* part_acc;
   unsigned long long wait_ns;  // bound of every mbarrier wait
   int inject;                  // test hook: 1 = each CTA's producer withholds its first stage
 };
@@ -842,6 +847,11 @@ __global__ void __launch_bounds__(THREADS, KvCfg<KV, D, CP>::MINB) decode_split_
     for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
       long long t0;
       if (seq_len<LAYOUT>(p, b, &t0) == 0) {
+        if (LAYOUT == PAGED && p.part_ml != nullptr) {
+          for (int qh = et; qh < p.q_heads; qh += ETHREADS)
+            p.part_ml[static_cast<long long>(b) * p.q_heads + qh] = make_float2(NEG_INF, 0.f);
+          continue;
+        }
         for (int qh = 0; qh < p.q_heads; ++qh)
           for (int d = et; d < D; d += ETHREADS)
             store_out(p, static_cast<long long>(b) * p.o_sb + static_cast<long long>(qh) * p.o_sh + d, 0.f);
@@ -916,7 +926,13 @@ __global__ void __launch_bounds__(THREADS, KvCfg<KV, D, CP>::MINB) decode_split_
         }
         const int qh = item_q<HP>(p, mt.h, hh, hd);
         const int hs = hh * GPAD + hd;  // head slot in a segment record
-        if (whole) {
+        if (LAYOUT == PAGED && whole && p.part_ml != nullptr) {
+          const long long pr = static_cast<long long>(mt.b) * p.q_heads + qh;
+          float4* dst = reinterpret_cast<float4*>(p.part_acc + pr * D + d4);
+#pragma unroll
+          for (int k = 0; k < D / 32; ++k) dst[8 * k] = A[k];
+          if ((u & 7) == 0) p.part_ml[pr] = make_float2(M, L);
+        } else if (whole) {
           float e, Lf;
           sink_norm(L, M, p.s_aux, qh, &e, &Lf);
           const long long ob = obase + static_cast<long long>(qh) * p.o_sh + d4;
@@ -1000,6 +1016,14 @@ __global__ void __launch_bounds__(THREADS, KvCfg<KV, D, CP>::MINB) decode_split_
           M = Mn;
         }
         const int qh = item_q<HP>(p, mt.h, hh, hd);
+        if (LAYOUT == PAGED && p.part_ml != nullptr) {
+          const long long pr = static_cast<long long>(mt.b) * p.q_heads + qh;
+          float4* dst = reinterpret_cast<float4*>(p.part_acc + pr * D + d0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) dst[i] = make_float4(A[4 * i], A[4 * i + 1], A[4 * i + 2], A[4 * i + 3]);
+          if (d0 == 0) p.part_ml[pr] = make_float2(M, L);
+          continue;
+        }
         const long long ob = obase + static_cast<long long>(qh) * p.o_sh + d0;
         float e, Lf;
         sink_norm(L, M, p.s_aux, qh, &e, &Lf);

@@ -244,6 +244,48 @@ typedef struct fk_rope_args {
 int fk_qk_norm_rope(const fk_rope_args* args, void* stream);
 
 /*
+ * Decode attention of a batch whose sequences share a prefix (no counterpart in
+ * the reference, which reads the prompt's pages once per sequence): query
+ * token b attends the prefix's tokens 0 .. prefix_len - 1 (page
+ * prefix_table[t / 16]) and then its own tokens 0 .. seq_lens[b] - 1 (page
+ * block_table[b, t / 16]), both in the same pools, with the sink formula of
+ * the other entries over the whole.  The prefix is read once for the batch and
+ * multiplied on the tensor cores.  A row with nothing to attend is zero.
+ * Types, scales, strides and alignment as fk_paged_flash_decode.
+ *
+ * prefix_len_dev (int32 on the device) is read when non-null, else prefix_len
+ * is used.  Prefix tokens past prefix_blocks * 16, or in a page outside
+ * [0, num_pages), are masked and set FK_STATUS_BAD_PAGE in *status (when
+ * non-null), as the own tokens' bad pages do.
+ *
+ * The workspace (fk_shared_prefix_workspace_bytes, 256-byte aligned) is pure
+ * scratch: it needs no initial value and carries nothing from call to call, so
+ * calls that may overlap only need buffers of their own.  Three kernels are
+ * queued on `stream`.
+ */
+typedef struct fk_prefix_args {
+  const void* q;              /* [batch, q_heads, D] */
+  const void* k_pool;         /* [num_pages, kv_heads, 16, D] */
+  const void* v_pool;
+  const void* prefix_table;   /* int32 [prefix_blocks] */
+  const void* prefix_len_dev; /* int32, or null */
+  const void* block_table;    /* int32 [batch, max_blocks] */
+  const void* seq_lens;       /* int32 [batch] */
+  const void* s_aux;          /* float [q_heads] or null */
+  void* out;                  /* [batch, q_heads, D] */
+  const void* scale_q;
+  const void* scale_k;
+  const void* scale_v;
+  void* status;               /* int32 or null */
+  int64_t prefix_len, prefix_blocks, batch, q_heads, kv_heads, head_dim, num_pages, max_blocks;
+  int64_t q_dtype, kv_dtype, out_dtype;
+  int64_t q_b, q_h, kp_p, kp_h, kp_s, vp_p, vp_h, vp_s, bt_b, o_b, o_h;
+} fk_prefix_args;
+
+size_t fk_shared_prefix_workspace_bytes(int device, int batch, int q_heads, int kv_heads, int head_dim, int kv_dtype);
+int fk_paged_shared_prefix_decode(const fk_prefix_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Measurement hooks (no reference counterpart: the reference times with
  * torch.profiler / triton.testing.do_bench, benchmarks/benchmark.py:87-91).
  * fk_profile_begin(n) records CUDA events on the launching stream just before

@@ -58,3 +58,19 @@ def shared_prefix_ref(q, kp, vp, prefix, kt, vt, lens, sink=None):
             w = torch.softmax(x, -1)[:, :k.shape[0]]
             out[b, h * G:(h + 1) * G] = w @ v
     return out
+
+
+def attention_bound(q, kp, vp, prefix, kt, vt, lens, sink, ref, p_dtype, out_dtype):
+    """How far shared-prefix attention may be from ref, relative to sum w |v|.
+    The softmax numerators are rounded to p_dtype (half a step each), the result
+    to out_dtype.  In 32 bits: logits (2^-22 of sum |q k| / sqrt(D), which is
+    under 64 in these tests: 2^-16), exponents (2^-24 of up to 64: 2^-18, times
+    ln 2), ex2 (2^-22); the sum over P tokens 16 at a time (2^-24 a step), the
+    numerators that vanish in f16 (under 2^-32 of the largest's for the prefix,
+    2^-25 for own tokens)."""
+    amp = shared_prefix_ref(q, kp, vp.abs(), prefix, kt, vt.abs(), lens, sink)
+    u, uo = torch.finfo(p_dtype).eps / 2, torch.finfo(out_dtype).eps / 2
+    tiny = 2.0 ** -25 if out_dtype == torch.float16 else 0.0
+    own = kt.shape[2]
+    f32 = 2.0 ** -15 + (prefix + own) / 16 * 2.0 ** -24 + prefix * 2.0 ** -32 + own * 2.0 ** -25
+    return (u + f32) * amp * (1 + uo) + uo * ref.abs() + tiny
