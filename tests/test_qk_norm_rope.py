@@ -122,7 +122,8 @@ def _inside(got, ref, amp):
 @pytest.mark.parametrize("D,R,il", [(128, 128, False), (128, 128, True), (128, 96, False), (128, 16, False), (64, 64, False),
                                     (64, 32, True), (64, 48, False), (128, 0, False)])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-@pytest.mark.parametrize("T,QH,KVH,norm", [(1, 1, 1, True), (7, 32, 8, True), (511, 5, 1, False), (513, 71, 3, True)])
+@pytest.mark.parametrize("T,QH,KVH,norm", [(1, 1, 1, True), (7, 32, 8, True), (511, 5, 1, False), (513, 71, 3, True),
+                                            (1023, 4, 2, True), (1024, 4, 2, True), (2777, 9, 3, True), (1500, 3, 1, False)])
 def test_norm_rope_matches_reference(dev, D, R, il, dtype, T, QH, KVH, norm):
     q, k, _ = _heads(dev, T, QH, KVH, D, dtype, seed=T + D + R)
     qw, kw = _weights(dev, D, dtype, T) if norm else (None, None)
@@ -212,6 +213,32 @@ def test_norm_rope_empty_and_bad_positions(dev):
     for t in (0, 2):
         _inside(qo[t], ref[t], amp[t])
     assert bool((qo[[1, 3, 4]] == 0).all()) and bool((ko[[1, 3, 4]] == 0).all())
+    assert int(st) == N.FK_STATUS_BAD_POSITION
+
+
+@gpu
+@pytest.mark.parametrize("T", [7, 3000])
+@pytest.mark.parametrize("layout", ["heads first", "in place", "wide"])
+def test_norm_rope_layouts_and_bad_positions_among_many(dev, T, layout):
+    """Few and many tokens take different kernels: rows that do not lie one
+    after another, outputs over inputs, a token too wide to stream."""
+    QH, KVH = (300, 150) if layout == "wide" else (8, 2)
+    q, k, _ = _heads(dev, T, QH, KVH, 128, torch.float16, seed=13)
+    cos, sin = fk.rope_table(500, 128, device=dev)
+    pos = torch.randint(0, 500, (T,), device=dev, dtype=torch.int32)
+    pos[::5] = -1
+    pos[3] = 500
+    w = _weights(dev, 128, torch.float16, 1)
+    st = torch.zeros(1, dtype=torch.int32, device=dev)
+    ok = (pos >= 0) & (pos < 500)
+    refs = [norm_rope_ref(x, cos, sin, pos.clamp(0, 499), w[i]) for i, x in enumerate((q, k))]
+    if layout == "heads first":
+        q, k = (x.transpose(0, 1).contiguous().transpose(0, 1) for x in (q, k))
+    out = (q, k) if layout == "in place" else (None, None)
+    qo, ko = fk.qk_norm_rope(q, k, cos, sin, pos, q_weight=w[0], k_weight=w[1], q_out=out[0], k_out=out[1], status=st)
+    for got, (ref, amp) in zip((qo, ko), refs):
+        _inside(got[ok], ref[ok], amp[ok])
+        assert bool((got[~ok] == 0).all())
     assert int(st) == N.FK_STATUS_BAD_POSITION
 
 
@@ -310,7 +337,8 @@ def _inside_e4m3(got, ref, amp):
 @pytest.mark.parametrize("pool", ["same", "e4m3"])
 @pytest.mark.parametrize("D,R,il,dtype", [(128, 128, False, torch.bfloat16), (128, 64, True, torch.float16),
                                           (64, 64, False, torch.float16), (64, 16, False, torch.bfloat16)])
-@pytest.mark.parametrize("counts,starts", [([1] * 5, [0, 15, 16, 333, 31]), ([1], [0]), ([3, 40, 1, 700], [14, 0, 47, 5])])
+@pytest.mark.parametrize("counts,starts", [([1] * 5, [0, 15, 16, 333, 31]), ([1], [0]), ([3, 40, 1, 700], [14, 0, 47, 5]),
+                                           ([1, 900, 2, 333, 600], [15, 7, 0, 1000, 1])])
 def test_append_rope_matches_reference(dev, pool, D, R, il, dtype, counts, starts):
     QH, KVH = 6, 3
     T = sum(counts)
