@@ -29,11 +29,15 @@
 // device from the prefix length.
 //
 // Warps: 0-3 and 4-7 softmax of stream 0 and 1 (thread = row), 8-11 load Q, K
-// and V, 12 issues the MMAs.  Loads are cp.async (16-bit) or loads widened to
-// f16 in registers (e4m3) rather than TMA: pages are 16 tokens, and a K or V
-// tile that the tensor cores read with one descriptor needs its 8-row groups
-// evenly spaced, which a page-sized box of two 128-byte halves does not leave;
-// cp.async also writes zeros for tokens past the prefix and for bad pages.
+// and V, 12 issues the MMAs.  A tile that the tensor cores read with one
+// descriptor needs its 8-row groups evenly spaced, so a page is loaded as one
+// box per 128-byte half, straight into its 16 rows of that half.  Each loader
+// warp loads two of a tile's eight pages: one warp issues a box in 100 to 150
+// cycles, and a tile's K and V are 32 boxes for 1024 to 2048 cycles of tensor
+// work.  e4m3 pages land in a ring of the warp's own and are widened to f16
+// from there.  Tiles that end the prefix or hold a bad page are loaded row by
+// row instead, with zeros where there is no token (the tail of a page may hold
+// anything, and 0 x NaN would reach the output).
 #include <cuda_fp8.h>
 
 #include "fk_decode_kernel.cuh"
@@ -48,17 +52,19 @@ constexpr int PTOK = 128;     // tokens of a token tile (MMA N of QK, K of PV)
 constexpr int PPAGES = PTOK / PAGE;
 constexpr int PTHREADS = 13 * 32;
 constexpr int HALF_BYTES = PTOK * 128;  // 128 rows of a 128-byte half
-constexpr int LOAD_LAG = 2;   // K / V tiles a loader issues ahead of the one it publishes
 
-template <int D>
+template <int KV, int D>
 struct PCfg {
+  static constexpr bool FP8 = KV == FK_DTYPE_E4M3;
   static constexpr int NH = D / 64;
   static constexpr int TILE_BYTES = NH * HALF_BYTES;  // Q, K or V tile in 16 bits
-  static constexpr int STAGES = D == 128 ? 5 : 8;
-  static constexpr int SMEM = 1024 + (2 + STAGES) * TILE_BYTES + 512;
+  static constexpr int STAGES = D == 64 ? 8 : FP8 ? 3 : 5;
+  static constexpr int RAW = FP8 ? 4 : 0;             // e4m3 tiles on the way
+  static constexpr int SMEM = 1024 + (2 + STAGES) * TILE_BYTES + RAW * HALF_BYTES;
 };
 
 struct PrefixParams {
+  CUtensorMap tk, tv;  // boxes of one page's 16 rows x 128 bytes
   const void* q;
   long long q_b, q_h;
   const void* k;
@@ -170,7 +176,7 @@ __device__ __forceinline__ uint4 load_q8(const PrefixParams& p, long long e, flo
 
 template <int KV, int D>
 __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_constant__ PrefixParams p) {
-  using C = PCfg<D>;
+  using C = PCfg<KV, D>;
   constexpr bool FP8 = KV == FK_DTYPE_E4M3;
   constexpr bool MBF16 = KV == FK_DTYPE_BF16;
   constexpr int ST = C::STAGES;
@@ -183,6 +189,9 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t sQ = smem;                           // [2] row tiles
   const uint32_t sKV = smem + 2 * C::TILE_BYTES;      // [ST]
+  const uint32_t sRaw = sKV + ST * C::TILE_BYTES;     // [RAW][loader warp] two e4m3 pages
+  constexpr int RAW = C::RAW > 0 ? C::RAW : 1;
+  __shared__ __align__(8) uint64_t b_raw[4][RAW];
   __shared__ __align__(8) uint64_t b_full[ST], b_empty[ST], b_qfull, b_qempty, b_s[2], b_p[2], b_o[2], b_drain;
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_bad;  // a bad page was seen: the softmax checks pages from then on
@@ -201,6 +210,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
       mbar_init(smem_u32(&b_o[i]), 1);
     }
     mbar_init(smem_u32(&b_drain), 1);
+    for (int i = 0; i < 4 * RAW; ++i) mbar_init(smem_u32(&b_raw[0][0] + i), 1);
     fence_mbar_init();
     s_bad = 0;
   }
@@ -380,148 +390,228 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
     }
   } else if (warp < 12) {
     // ============================================================ loaders
-    const int lt = tid - 256;
-    int stage = 0, pstage = 0, pending = 0;
+    const int lw = warp - 8, lt = tid - 256;
+    int stage = 0;
     uint32_t eph = 1, qph = 1;
     const float sq = p.scale_q != nullptr ? __ldg(p.scale_q) : 1.f;
     const uint32_t flip = sk < 0.f ? 0x80008000u : 0u;  // a negative scale turns Q over: the softmax sees |scale|
     bool alive = true;
     bool withhold = p.inject == 1;
-    auto publish = [&]() {  // the oldest unpublished tile is in shared memory
-      fence_async_proxy();
-      __syncwarp();
-      if (lane == 0 && !withhold) mbar_arrive(smem_u32(&b_full[pstage]));
-      withhold = false;
-      if (++pstage == ST) pstage = 0;
-      --pending;
-    };
-    // page of the tile that this lane looks up
+    uint32_t raw_par = 0;  // parity of each raw slot's next completion
+    uint32_t armed = 0, armed_par = 0;  // stages this warp has armed with copies, and the parity each was armed in
+    if (lane == 0) {
+      prefetch_tmap(&p.tk);
+      prefetch_tmap(&p.tv);
+    }
+    // A tile's pages, one per lane (8 distinct), and whether a plain load of all
+    // of them is right: every page in the pool, every token before the end.
     auto lookup = [&](int tile) -> int {
       const int pg = tile * PPAGES + (lane & 7);
-      return pg < p.blocks ? __ldg(p.table + pg) : -1;
+      const int ph = pg < p.blocks ? __ldg(p.table + pg) : -1;
+      return ph < p.num_pages ? ph : -1;
+    };
+    auto plain = [&](int tile, int ent) -> bool { return (tile + 1) * PTOK <= plen && __all_sync(0xffffffffu, ent >= 0); };
+    auto advance = [&]() {
+      if (++stage == ST) {
+        stage = 0;
+        eph ^= 1u;
+      }
     };
     for (long long g = g0; g < g1 && alive;) {
       PrefixSeg sg;
       g += prefix_segment(pl, g, g1, blockIdx.x, &sg);
+      const int items = 2 * sg.tiles;
       bool is_v;
       int tile = sg.t0 + load_item(0, sg.tiles, sg.dual, &is_v);
       int ent = lookup(tile);
-      // ---- Q: the unit's row tiles, once the previous segment's products are done
-      if (!FP8) {
-        cp_async_wait<0>();
-        while (pending > 0) publish();
-      }
+      // ---- Q: the unit's row tiles, once the previous segment's products are
+      // done; Q of the MMA's type with aligned rows is copied asynchronously
+      // while the first tile is requested
       if (!(alive = wait(&b_qempty, qph))) break;
       qph ^= 1u;
-#pragma unroll 1
-      for (int s = 0; s < (sg.dual ? 2 : 1); ++s) {
+      const bool q_async = p.q_al16 != 0 && p.q_dtype == (MBF16 ? FK_DTYPE_BF16 : FK_DTYPE_F16) && flip == 0;
+      {
         constexpr int CPR = D / 8;  // 16-byte chunks of a row
-#pragma unroll 4
-        for (int u = lt; u < PROWS * CPR; u += 128) {
-          const int r = u / CPR, ch = u % CPR;
-          const int grow = (2 * sg.unit + s) * PROWS + r;
-          uint4 x = make_uint4(0u, 0u, 0u, 0u);
-          if (grow < p.rows) {
+        const int ch = lt % CPR;
+#pragma unroll 1
+        for (int s = 0; s < (sg.dual ? 2 : 1); ++s) {
+          const uint32_t dst = sQ + s * C::TILE_BYTES + (ch >> 3) * HALF_BYTES;
+#pragma unroll 8
+          for (int r = lt / CPR; r < PROWS; r += 128 / CPR) {
+            const int grow = (2 * sg.unit + s) * PROWS + r;
             const int b = grow / p.G, gg = grow - b * p.G;
-            x = load_q8<MBF16>(p, b * p.q_b + static_cast<long long>(sg.h * p.G + gg) * p.q_h + ch * 8, sq, flip);
+            const long long e = b * p.q_b + static_cast<long long>(sg.h * p.G + gg) * p.q_h + ch * 8;
+            const uint32_t d = dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+            const bool in = grow < p.rows;
+            if (q_async) {
+              cp_async16_zfill(d, static_cast<const unsigned short*>(p.q) + (in ? e : 0), in);
+            } else {
+              const uint4 x = in ? load_q8<MBF16>(p, e, sq, flip) : make_uint4(0u, 0u, 0u, 0u);
+              sts128(d, x.x, x.y, x.z, x.w);
+            }
           }
-          sts128(sQ + s * C::TILE_BYTES + (ch >> 3) * HALF_BYTES + r * 128 + (((ch & 7) ^ (r & 7)) << 4), x.x, x.y, x.z, x.w);
         }
+        cp_async_commit();
       }
-      fence_async_proxy();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&b_qfull));
+      auto publish_q = [&]() {
+        cp_async_wait<0>();
+        fence_async_proxy();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&b_qfull));
+      };
 
       // ---- K and V tiles
       if constexpr (!FP8) {
-        constexpr int CPR = D / 8, RPS = 128 / CPR;  // chunks of a row, rows per step of the 128 threads
-        const int r0 = lt / CPR, ch = lt % CPR;
-        for (int idx = 0; idx < 2 * sg.tiles; ++idx) {
+        for (int idx = 0; idx < items; ++idx) {
           const int t = tile, e = ent;
           const bool v = is_v;
-          if (idx + 1 < 2 * sg.tiles) {
+          if (idx + 1 < items) {
             tile = sg.t0 + load_item(idx + 1, sg.tiles, sg.dual, &is_v);
             ent = lookup(tile);
           }
           if (!(alive = wait(&b_empty[stage], eph))) break;
-          const char* base = static_cast<const char*>(v ? p.v : p.k);
-          const long long sp = (v ? p.vp_p : p.kp_p) * 2, ss = (v ? p.vp_s : p.kp_s) * 2;
-          const char* hb = base + (v ? p.vp_h : p.kp_h) * 2 * sg.h + ch * 16;
-          const uint32_t dst = sKV + stage * C::TILE_BYTES + (ch >> 3) * HALF_BYTES;
+          const uint32_t full = smem_u32(&b_full[stage]);
+          const uint32_t dst = sKV + stage * C::TILE_BYTES;
+          const bool all = plain(t, e);
+          const int ph0 = __shfl_sync(0xffffffffu, e, 2 * lw), ph1 = __shfl_sync(0xffffffffu, e, 2 * lw + 1);
+          if (withhold) {
+            withhold = false;
+          } else if (all) {
+            if (lane == 0) {
+              const CUtensorMap* map = v ? &p.tv : &p.tk;
+              const uint32_t d0 = dst + 2 * lw * 2048;
+              mbar_arrive_expect_tx(full, 2 * C::NH * 2048);
 #pragma unroll
-          for (int k = 0; k < PTOK / RPS; ++k) {
-            const int r = r0 + k * RPS;
-            const int ph = __shfl_sync(0xffffffffu, e, (k * RPS) >> 4);
-            const bool okp = ph >= 0 && ph < p.num_pages;
-            const bool ok = okp && t * PTOK + r < plen;
-            if (!okp && t * PTOK + ((k * RPS) & ~15) < plen) s_bad = 1;
-            cp_async16_zfill(dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4), ok ? hb + ph * sp + (r & 15) * ss : base, ok);
+              for (int hf = 0; hf < C::NH; ++hf) {
+                tma_load_5d(d0 + hf * HALF_BYTES, map, full, 0, 0, hf, sg.h, ph0);
+                tma_load_5d(d0 + hf * HALF_BYTES + 2048, map, full, 0, 0, hf, sg.h, ph1);
+              }
+            }
+            armed |= 1u << stage;
+            armed_par = (armed_par & ~(1u << stage)) | ((eph ^ 1u) << stage);
+          } else {
+            // this warp's 32 rows, 16 bytes at a time
+            constexpr int CPR = D / 8;
+            const char* base = static_cast<const char*>(v ? p.v : p.k) + (v ? p.vp_h : p.kp_h) * 2 * sg.h;
+            const long long sp = (v ? p.vp_p : p.kp_p) * 2, ss = (v ? p.vp_s : p.kp_s) * 2;
+#pragma unroll 4
+            for (int u = lane; u < 32 * CPR; u += 32) {
+              const int r = u / CPR, ch = u % CPR, tok = t * PTOK + 32 * lw + r;
+              const int ph = r < 16 ? ph0 : ph1;
+              const bool ok = ph >= 0 && tok < plen;
+              if (ph < 0 && tok < plen) s_bad = 1;
+              const int row = 32 * lw + r;
+              cp_async16_zfill(dst + (ch >> 3) * HALF_BYTES + row * 128 + (((ch & 7) ^ (row & 7)) << 4),
+                               ok ? base + ph * sp + (r & 15) * ss + ch * 16 : base, ok);
+            }
+            cp_async_commit();
+            cp_async_wait<0>();
+            fence_async_proxy();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full);
           }
-          cp_async_commit();
-          ++pending;
-          if (++stage == ST) {
-            stage = 0;
-            eph ^= 1u;
-          }
-          if (pending > LOAD_LAG) {
-            cp_async_wait<LOAD_LAG>();
-            publish();
-          }
+          advance();
+          if (idx == 0) publish_q();
         }
       } else {
-        // e4m3: 16 bytes of a row per load, widened to two 16-byte chunks of f16;
-        // the next tile's loads are in flight while this one is widened
-        constexpr int NL = 8;  // loads of a thread per tile: 128 rows x 8 chunks / 128
-        const int r0 = lt >> 3, ch = lt & 7;
-        uint4 buf[NL];
-        auto fetch = [&](int t, bool v, int e) {
-          const unsigned char* base = static_cast<const unsigned char*>(v ? p.v : p.k);
-          const long long sp = v ? p.vp_p : p.kp_p;
-          const unsigned char* hb = base + (v ? p.vp_h : p.kp_h) * sg.h + ch * 16 + r0 * (v ? p.vp_s : p.kp_s);
+        // e4m3: raw pages RAW - 1 tiles ahead; this warp widens its own 32 rows
+        const uint32_t raw0 = sRaw + lw * 4096;
+        // what is on the way: item, its pages, whether a TMA brings it
+        int rt = tile;         // tile of the next request
+        bool rv = is_v;
+        int rent = ent;
+        int req = 0;           // items requested
+        int qt[RAW], qph0[RAW], qph1[RAW];
+        bool qv[RAW], qall[RAW];
 #pragma unroll
-          for (int k = 0; k < NL; ++k) {
-            const int ph = __shfl_sync(0xffffffffu, e, k);
-            const bool okp = ph >= 0 && ph < p.num_pages;
-            if (!okp && t * PTOK + k * 16 < plen) s_bad = 1;
-            buf[k] = make_uint4(0u, 0u, 0u, 0u);
-            if (okp && t * PTOK + k * 16 + r0 < plen) buf[k] = __ldg(reinterpret_cast<const uint4*>(hb + ph * sp));
+        for (int i = 0; i < RAW; ++i) qt[i] = qph0[i] = qph1[i] = 0, qv[i] = qall[i] = false;
+        auto request = [&](int slot) {  // slot = req % RAW, a constant
+          qt[slot] = rt;
+          qv[slot] = rv;
+          qall[slot] = plain(rt, rent);
+          qph0[slot] = __shfl_sync(0xffffffffu, rent, 2 * lw);
+          qph1[slot] = __shfl_sync(0xffffffffu, rent, 2 * lw + 1);
+          if (qall[slot] && lane == 0) {
+            const CUtensorMap* map = rv ? &p.tv : &p.tk;
+            const uint32_t bar = smem_u32(&b_raw[lw][slot]);
+            mbar_arrive_expect_tx(bar, 4096);
+            tma_load_4d(raw0 + slot * HALF_BYTES, map, bar, 0, 0, sg.h, qph0[slot]);
+            tma_load_4d(raw0 + slot * HALF_BYTES + 2048, map, bar, 0, 0, sg.h, qph1[slot]);
+          }
+          if (++req < items) {
+            rt = sg.t0 + load_item(req, sg.tiles, sg.dual, &rv);
+            rent = lookup(rt);
           }
         };
-        fetch(tile, is_v, ent);
-        for (int idx = 0; idx < 2 * sg.tiles; ++idx) {
-          uint4 cur[NL];
 #pragma unroll
-          for (int k = 0; k < NL; ++k) cur[k] = buf[k];
-          if (idx + 1 < 2 * sg.tiles) {
-            tile = sg.t0 + load_item(idx + 1, sg.tiles, sg.dual, &is_v);
-            fetch(tile, is_v, lookup(tile));
-          }
-          if (!(alive = wait(&b_empty[stage], eph))) break;
-          const uint32_t dst = sKV + stage * C::TILE_BYTES + (ch >> 2) * HALF_BYTES;
+        for (int i = 0; i < RAW - 1; ++i)
+          if (req < items) request(i);
+        publish_q();
+        for (int i0 = 0; i0 < items && alive; i0 += RAW) {
 #pragma unroll
-          for (int k = 0; k < NL; ++k) {
-            const int r = r0 + k * 16;
-            uint32_t w[8];
-            e4m3x4_to_f16x2x2(cur[k].x, w[0], w[1]);
-            e4m3x4_to_f16x2x2(cur[k].y, w[2], w[3]);
-            e4m3x4_to_f16x2x2(cur[k].z, w[4], w[5]);
-            e4m3x4_to_f16x2x2(cur[k].w, w[6], w[7]);
+          for (int sl = 0; sl < RAW; ++sl) {
+            const int idx = i0 + sl;
+            if (idx >= items) break;
+            // the slot that the previous item left is requested anew
+            if (req < items) request((sl + RAW - 1) % RAW);
+            const int t = qt[sl], ph0 = qph0[sl], ph1 = qph1[sl];
+            // lane: rows (lane >> 3) + 4 k, 16-byte chunk lane & 7 (16 elements)
+            const int ch = lane & 7, r0 = lane >> 3;
+            uint4 x[8];
+            if (qall[sl]) {
+              if (!(alive = wait(&b_raw[lw][sl], (raw_par >> sl) & 1u))) break;
+              raw_par ^= 1u << sl;
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const int r = r0 + 4 * k;
+                x[k] = lds128(raw0 + sl * HALF_BYTES + r * 128 + ((ch ^ (r & 7)) << 4));
+              }
+            } else {
+              const unsigned char* base = static_cast<const unsigned char*>(qv[sl] ? p.v : p.k) + (qv[sl] ? p.vp_h : p.kp_h) * sg.h;
+              const long long sp = qv[sl] ? p.vp_p : p.kp_p, ss = qv[sl] ? p.vp_s : p.kp_s;
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const int r = r0 + 4 * k, tok = t * PTOK + 32 * lw + r;
+                const int ph = r < 16 ? ph0 : ph1;
+                if (ph < 0 && tok < plen) s_bad = 1;
+                x[k] = make_uint4(0u, 0u, 0u, 0u);
+                if (ph >= 0 && tok < plen) x[k] = __ldg(reinterpret_cast<const uint4*>(base + ph * sp + (r & 15) * ss + ch * 16));
+              }
+            }
+            if (!(alive = wait(&b_empty[stage], eph))) break;
+            const uint32_t dst = sKV + stage * C::TILE_BYTES + (ch >> 2) * HALF_BYTES + 32 * lw * 128;
             const int c0 = (2 * ch) & 7;
-            sts128(dst + r * 128 + ((c0 ^ (r & 7)) << 4), w[0], w[1], w[2], w[3]);
-            sts128(dst + r * 128 + (((c0 + 1) ^ (r & 7)) << 4), w[4], w[5], w[6], w[7]);
-          }
-          ++pending;
-          publish();
-          if (++stage == ST) {
-            stage = 0;
-            eph ^= 1u;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const int r = r0 + 4 * k;
+              uint32_t w[8];
+              e4m3x4_to_f16x2x2(x[k].x, w[0], w[1]);
+              e4m3x4_to_f16x2x2(x[k].y, w[2], w[3]);
+              e4m3x4_to_f16x2x2(x[k].z, w[4], w[5]);
+              e4m3x4_to_f16x2x2(x[k].w, w[6], w[7]);
+              sts128(dst + r * 128 + ((c0 ^ (r & 7)) << 4), w[0], w[1], w[2], w[3]);
+              sts128(dst + r * 128 + (((c0 + 1) ^ (r & 7)) << 4), w[4], w[5], w[6], w[7]);
+            }
+            // also orders the reads of the raw slot before its next copy
+            fence_async_proxy();
+            __syncwarp();
+            if (lane == 0 && !withhold) mbar_arrive(smem_u32(&b_full[stage]));
+            withhold = false;
+            advance();
           }
         }
       }
     }
-    cp_async_wait<0>();  // also on the way out after a wait that ran out
-    if (alive)
-      while (pending > 0) publish();
+    // A wait ran out: let the copies in flight land before the block exits.
+    cp_async_wait<0>();
+    if (!alive && lane == 0) {
+      if constexpr (FP8) {
+        for (int i = 0; i < RAW; ++i) mbar_wait(smem_u32(&b_raw[lw][i]), (raw_par >> i) & 1u, p.wait_ns);
+      } else {
+        for (int i = 0; i < ST; ++i)
+          if ((armed >> i) & 1u) mbar_wait(smem_u32(&b_full[i]), (armed_par >> i) & 1u, p.wait_ns);
+      }
+    }
     if (s_bad && lane == 0 && p.status != nullptr) atomicOr(p.status, FK_STATUS_BAD_PAGE);
   } else if (lane == 0) {
     // ============================================================ MMA issue (one thread)
@@ -640,8 +730,10 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
 
 // ------------------------------------------------------------------------
 // Join: out = (sum_i 2^(m_i - M) acc_i) / (sum_i 2^(m_i - M) l_i [+ 2^(s - M)])
-// over the prefix segments of the row and its own part.  Thread = row of a row
-// tile, 16 dims; the segments' records are read once, 512 bytes per warp.
+// over the prefix segments of the row and its own part, in one pass with a
+// running maximum.  A thread has one row and four dims and keeps eight records'
+// loads in flight; a warp reads 512 contiguous bytes of a record.  With fewer
+// rows than threads the block takes more dims instead.
 // ------------------------------------------------------------------------
 struct JoinParams {
   const float2* ml;       // prefix segments
@@ -654,94 +746,103 @@ struct JoinParams {
   const float* scale_v;
   void* out;
   long long o_b, o_h;
-  int out_dtype, o_al16;
+  int out_dtype, o_al8;
   const int* own_status;
   int* status;
+  int rb;  // rows of a block (a power of two); JTHREADS / rb groups of four dims
 };
 
-constexpr int JDIMS = 16;
+constexpr int JTHREADS = 128;
+constexpr int JBATCH = 8;
 
 template <int D>
-__global__ void __launch_bounds__(PROWS) join_kernel(const __grid_constant__ JoinParams p) {
+__global__ void __launch_bounds__(JTHREADS) join_kernel(const __grid_constant__ JoinParams p) {
   grid_dependency_wait();
   grid_dependency_trigger();
   if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0 && p.status != nullptr && *p.own_status != 0)
     atomicOr(p.status, *p.own_status);
-  const int rt = (p.rows + PROWS - 1) / PROWS;
-  const int h = blockIdx.x / rt, tile = blockIdx.x % rt;
-  const int row = threadIdx.x, grow = tile * PROWS + row;
-  if (grow >= p.rows) return;
+  const int per_head = (p.rows + p.rb - 1) / p.rb;
+  const int h = blockIdx.x / per_head, first = blockIdx.x % per_head * p.rb;  // the block's first row
+  const int tile = first / PROWS, row = first % PROWS + (threadIdx.x & (p.rb - 1));
+  const int grow = tile * PROWS + row;
+  const int d0 = (blockIdx.y * (JTHREADS / p.rb) + threadIdx.x / p.rb) * 4;
+  if (grow >= p.rows || d0 >= D) return;
   const int b = grow / p.G, qh = h * p.G + grow % p.G;
-  const int d0 = blockIdx.y * JDIMS;
+  const long long orow = static_cast<long long>(b) * p.q_heads + qh;
+  const float2 own = __ldcg(p.own_ml + orow);
+  const float4 own_a = __ldcg(reinterpret_cast<const float4*>(p.own_acc + orow * D + d0));
   const int plen = max(p.plen_dev != nullptr ? __ldg(p.plen_dev) : p.plen, 0);
   const PrefixPlan pl(plen, p.rows, p.kv_heads, p.ctas);
   const int unit = tile >> 1;
   const bool dual = unit < pl.nd;
-  int s0 = 0, ns = 0;  // records: stream st of segment s0 + i is record 2 (s0 + i) + st
+  long long rec0 = 0;  // the row's records: every (dual) second one from rec0 on
+  int nrec = 0;
   if (pl.nt > 0) {
     const long long base = h * pl.gh + pl.unit_base(unit);
     const long long c0 = base / pl.per, c1 = (base + pl.unit_len(unit) - 1) / pl.per;
-    s0 = static_cast<int>(c0) + h * pl.upu + unit;
-    ns = static_cast<int>(c1 - c0) + 1;
+    rec0 = 2 * (c0 + h * pl.upu + unit) + (dual ? (tile & 1) : 0);
+    nrec = static_cast<int>(c1 - c0 + 1) * (dual ? 1 : 2);
   }
-  const int nrec = dual ? ns : 2 * ns;
-  auto rec_of = [&](int i) -> long long { return dual ? 2ll * (s0 + i) + (tile & 1) : 2ll * s0 + i; };
+  const int rstep = dual ? 2 : 1;
 
-  const long long orow = static_cast<long long>(b) * p.q_heads + qh;
-  const float2 own = __ldcg(p.own_ml + orow);
-  float M = own.x;
-  for (int i = 0; i < nrec; ++i) M = fmaxf(M, __ldcg(p.ml + rec_of(i) * PROWS + row).x);
-  float L = 0.f;
-  if (p.s_aux != nullptr) {
-    const float s2 = __ldg(p.s_aux + qh) * LOG2E;
-    M = fmaxf(M, s2);
-    if (M != NEG_INF) L = exp2f(s2 - M);
-  }
-  float A[JDIMS];
-#pragma unroll
-  for (int i = 0; i < JDIMS; ++i) A[i] = 0.f;
-  auto add = [&](float e, float4 v, int k) {
-    A[4 * k] += e * v.x;
-    A[4 * k + 1] += e * v.y;
-    A[4 * k + 2] += e * v.z;
-    A[4 * k + 3] += e * v.w;
-  };
+  float M = NEG_INF, L = 0.f;
+  float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+  // a part with nothing in it (max -inf) may have unwritten accumulators
   if (own.x != NEG_INF) {
-    const float e = exp2f(own.x - M);
-    L += e * own.y;
-#pragma unroll
-    for (int k = 0; k < JDIMS / 4; ++k) add(e, __ldcg(reinterpret_cast<const float4*>(p.own_acc + orow * D + d0) + k), k);
+    M = own.x;
+    L = own.y;
+    A = own_a;
   }
-#pragma unroll 4
-  for (int i = 0; i < nrec; ++i) {
-    const long long rec = rec_of(i);
-    const float2 ml = __ldcg(p.ml + rec * PROWS + row);
-    if (ml.x == NEG_INF) continue;  // nothing attended: its accumulators may be unwritten
-    const float e = exp2f(ml.x - M);
-    L += e * ml.y;
-    const float4* src = reinterpret_cast<const float4*>(p.acc + rec * PROWS * D) + (d0 / 4) * PROWS + row;
+  for (int i = 0; i < nrec; i += JBATCH) {
+    float2 ml[JBATCH];
+    float4 av[JBATCH];
 #pragma unroll
-    for (int k = 0; k < JDIMS / 4; ++k) add(e, __ldcg(src + k * PROWS), k);
-  }
-  const float sv = p.scale_v != nullptr ? __ldg(p.scale_v) : 1.f;
-  const long long ob = b * p.o_b + qh * p.o_h + d0;
-#pragma unroll
-  for (int i = 0; i < JDIMS; ++i) A[i] = norm_out(A[i], 1.f, L, sv);
-  const bool bf = p.out_dtype == FK_DTYPE_BF16;
-  if (p.o_al16) {
-#pragma unroll
-    for (int k = 0; k < JDIMS; k += 8) {
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        w[i] = bf ? pack2<true>(A[k + 2 * i], A[k + 2 * i + 1]) : pack2<false>(A[k + 2 * i], A[k + 2 * i + 1]);
-      *reinterpret_cast<uint4*>(static_cast<unsigned short*>(p.out) + ob + k) = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int k = 0; k < JBATCH; ++k) {
+      const bool ok = i + k < nrec;
+      const long long rec = rec0 + static_cast<long long>(ok ? i + k : i) * rstep;
+      ml[k] = __ldcg(p.ml + rec * PROWS + row);
+      av[k] = __ldcg(reinterpret_cast<const float4*>(p.acc + rec * PROWS * D) + (d0 / 4) * PROWS + row);
+      if (!ok) ml[k].x = NEG_INF;
     }
-  } else {
+    float Mn = M;
 #pragma unroll
-    for (int i = 0; i < JDIMS; ++i) {
-      if (bf) static_cast<__nv_bfloat16*>(p.out)[ob + i] = __float2bfloat16_rn(A[i]);
-      else static_cast<__half*>(p.out)[ob + i] = __float2half_rn(A[i]);
+    for (int k = 0; k < JBATCH; ++k) Mn = fmaxf(Mn, ml[k].x);
+    if (Mn == NEG_INF) continue;
+    const float sc = exp2f(M - Mn);
+    L *= sc;
+    A.x *= sc;
+    A.y *= sc;
+    A.z *= sc;
+    A.w *= sc;
+#pragma unroll
+    for (int k = 0; k < JBATCH; ++k) {
+      if (ml[k].x == NEG_INF) continue;
+      const float e = exp2f(ml[k].x - Mn);
+      L += e * ml[k].y;
+      A.x += e * av[k].x;
+      A.y += e * av[k].y;
+      A.z += e * av[k].z;
+      A.w += e * av[k].w;
+    }
+    M = Mn;
+  }
+  float e, Lf;
+  if (M == NEG_INF) e = 0.f, Lf = 0.f;  // nothing attended: zeros, whatever the sink
+  else sink_norm(L, M, p.s_aux, qh, &e, &Lf);
+  const float sv = p.scale_v != nullptr ? __ldg(p.scale_v) : 1.f;
+  const float o0 = norm_out(A.x, e, Lf, sv), o1 = norm_out(A.y, e, Lf, sv), o2 = norm_out(A.z, e, Lf, sv),
+              o3 = norm_out(A.w, e, Lf, sv);
+  const long long ob = b * p.o_b + qh * p.o_h + d0;
+  const bool bf = p.out_dtype == FK_DTYPE_BF16;
+  if (p.o_al8) {
+    *reinterpret_cast<uint2*>(static_cast<unsigned short*>(p.out) + ob) =
+        bf ? make_uint2(pack2<true>(o0, o1), pack2<true>(o2, o3)) : make_uint2(pack2<false>(o0, o1), pack2<false>(o2, o3));
+  } else {
+    const float o[4] = {o0, o1, o2, o3};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (bf) static_cast<__nv_bfloat16*>(p.out)[ob + i] = __float2bfloat16_rn(o[i]);
+      else static_cast<__half*>(p.out)[ob + i] = __float2half_rn(o[i]);
     }
   }
 }
@@ -782,12 +883,12 @@ int launch_prefix(const PrefixParams& p, int ctas, int device, cudaStream_t stre
   {
     std::lock_guard<std::mutex> lk(mu);
     if (!done[device]) {
-      const cudaError_t e = cudaFuncSetAttribute(prefix_kernel<KV, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, PCfg<D>::SMEM);
+      const cudaError_t e = cudaFuncSetAttribute(prefix_kernel<KV, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, PCfg<KV, D>::SMEM);
       if (e != cudaSuccess) return fail(FK_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
       done[device] = true;
     }
   }
-  const cudaError_t e = launch_pdl(prefix_kernel<KV, D>, dim3(ctas), dim3(PTHREADS), PCfg<D>::SMEM, stream, p);
+  const cudaError_t e = launch_pdl(prefix_kernel<KV, D>, dim3(ctas), dim3(PTHREADS), PCfg<KV, D>::SMEM, stream, p);
   return e == cudaSuccess ? FK_OK : fail(FK_ERR_CUDA, "prefix launch failed: %s", cudaGetErrorString(e));
 }
 
@@ -858,6 +959,25 @@ extern "C" int fk_paged_shared_prefix_decode(const fk_prefix_args* a, void* work
   p.zero_words = own_part_zero_words(own, w.own);
   p.status = static_cast<int*>(a->status);
   debug_settings(&p.wait_ns, &p.inject);
+  // 16-bit: (64 dims, 16 slots, D / 64 halves, heads, pages), a box is one
+  // half of a page; e4m3: (128 dims, 16 slots, heads, pages), a box is a page
+  for (int i = 0; i < 2; ++i) {
+    const void* base = i == 0 ? p.k : p.v;
+    const uint64_t sp = static_cast<uint64_t>(i == 0 ? p.kp_p : p.vp_p), sh = static_cast<uint64_t>(i == 0 ? p.kp_h : p.vp_h),
+                   ss = static_cast<uint64_t>(i == 0 ? p.kp_s : p.vp_s);
+    if (kv == FK_DTYPE_E4M3) {
+      const uint64_t dims[4] = {128, PAGE, static_cast<uint64_t>(KVH), static_cast<uint64_t>(a->num_pages)};
+      const uint64_t strides[3] = {ss, sh, sp};
+      const uint32_t box[4] = {128, PAGE, 1, 1};
+      rc = encode_map(i == 0 ? &p.tk : &p.tv, kv, 4, base, dims, strides, box);
+    } else {
+      const uint64_t dims[5] = {64, PAGE, static_cast<uint64_t>(D / 64), static_cast<uint64_t>(KVH), static_cast<uint64_t>(a->num_pages)};
+      const uint64_t strides[4] = {2 * ss, 128, 2 * sh, 2 * sp};
+      const uint32_t box[5] = {64, PAGE, 1, 1, 1};
+      rc = encode_map(i == 0 ? &p.tk : &p.tv, kv, 5, base, dims, strides, box);
+    }
+    if (rc != FK_OK) return rc;
+  }
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   DeviceScope scope(device);
   if (kv == FK_DTYPE_F16) rc = D == 64 ? launch_prefix<FK_DTYPE_F16, 64>(p, ctas, device, st) : launch_prefix<FK_DTYPE_F16, 128>(p, ctas, device, st);
@@ -884,12 +1004,13 @@ extern "C" int fk_paged_shared_prefix_decode(const fk_prefix_args* a, void* work
   j.o_b = a->o_b;
   j.o_h = a->o_h;
   j.out_dtype = static_cast<int>(a->out_dtype);
-  j.o_al16 = ((reinterpret_cast<uintptr_t>(a->out) & 15) == 0 && (a->o_b & 7) == 0 && (a->o_h & 7) == 0) ? 1 : 0;
+  j.o_al8 = own.p.o_al8;
   j.own_status = reinterpret_cast<const int*>(ws);
   j.status = p.status;
-  const int rt = (p.rows + PROWS - 1) / PROWS;
-  const dim3 grid(static_cast<unsigned>(KVH * rt), static_cast<unsigned>(D / JDIMS));
-  const cudaError_t e = D == 128 ? launch_pdl(join_kernel<128>, grid, dim3(PROWS), 0, st, j)
-                                 : launch_pdl(join_kernel<64>, grid, dim3(PROWS), 0, st, j);
+  j.rb = 8;
+  while (j.rb < PROWS && j.rb < p.rows) j.rb *= 2;
+  const dim3 grid(static_cast<unsigned>(KVH * ((p.rows + j.rb - 1) / j.rb)), static_cast<unsigned>((D / 4 * j.rb + JTHREADS - 1) / JTHREADS));
+  const cudaError_t e = D == 128 ? launch_pdl(join_kernel<128>, grid, dim3(JTHREADS), 0, st, j)
+                                 : launch_pdl(join_kernel<64>, grid, dim3(JTHREADS), 0, st, j);
   return e == cudaSuccess ? FK_OK : fail(FK_ERR_CUDA, "join launch failed: %s", cudaGetErrorString(e));
 }
