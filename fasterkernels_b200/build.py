@@ -22,7 +22,7 @@ LIB_PATH = os.path.join(LIB_DIR, "libfk_decode.so")
 SOURCES = [os.path.join(CSRC, n) for n in ("fk_decode.cu", "fk_kernels_f16.cu", "fk_kernels_bf16.cu",
                                            "fk_kernels_e4m3.cu", "fk_paged_append.cu", "fk_rope.cu", "fk_prefix.cu")]
 DEPS = SOURCES + [os.path.join(CSRC, "fk_ptx.cuh"), os.path.join(CSRC, "fk_decode_kernel.cuh"),
-                  os.path.join(CSRC, "fk_host.h"), os.path.join(CSRC, "fk_prefix.h"), os.path.join(CSRC, "fk_tc.cuh"),
+                  os.path.join(CSRC, "fk_host.h"), os.path.join(CSRC, "fk_prefix.h"), os.path.join(CSRC, "fk_tc.cuh"), os.path.join(CSRC, "fk_f32x2.cuh"),
                   os.path.join(REPO_DIR, "include", "fk_decode.h"), os.path.abspath(__file__)]
 
 NVCC_FLAGS = [

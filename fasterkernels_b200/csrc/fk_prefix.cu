@@ -47,10 +47,18 @@
 
 namespace fk {
 
+#ifndef PSHARE
+#define PSHARE 3
+#endif
+#ifndef RSOFT
+#define RSOFT 184
+#define RLOAD 96
+#define RMMA 48
+#endif
 constexpr int PROWS = 128;    // rows of a row tile (MMA M)
 constexpr int PTOK = 128;     // tokens of a token tile (MMA N of QK, K of PV)
 constexpr int PPAGES = PTOK / PAGE;
-constexpr int PTHREADS = 13 * 32;
+constexpr int PTHREADS = 16 * 32;  // four warpgroups (12-15: MMA issue, three idle warps)
 constexpr int HALF_BYTES = PTOK * 128;  // 128 rows of a 128-byte half
 
 template <int KV, int D>
@@ -215,10 +223,14 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
     s_bad = 0;
   }
   if (warp == 12) tmem_alloc(smem_u32(&s_tmem), 512);
+  if (tid == 8 * 32) {
+    prefetch_tmap(&p.tk);
+    prefetch_tmap(&p.tv);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *const_cast<volatile uint32_t*>(&s_tmem);
+  const uint32_t tmem = 0;  // all 512 columns are ours, so the allocation starts at column 0
   grid_dependency_wait();
   grid_dependency_trigger();
   for (int i = blockIdx.x * PTHREADS + tid; i < p.zero_words; i += gridDim.x * PTHREADS) p.zero[i] = 0;
@@ -240,6 +252,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
 
   if (warp < 8) {
     // ============================================================ softmax
+    reg_inc<RSOFT>();
     const int s = warp >> 2;
     const int row = tid & 127;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // lane (warp & 3) * 32 in bits 16..
@@ -275,35 +288,29 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
           for (int j = 0; j < 32; ++j)
             if (col + j >= lim || !((okp >> ((col + j) >> 4)) & 1u)) r[j] = __float_as_uint(NEG_INF);
         };
-        // ---- the row's maximum
-        uint32_t ra[32], rb[32];
+        // ---- the row of S, its maximum
+        uint32_t r[4][32];
+#pragma unroll
+        for (int ch = 0; ch < 4; ++ch) tmem_ld32(tS + 32 * ch, r[ch]);
         float mx0 = NEG_INF, mx1 = NEG_INF, mx2 = NEG_INF, mx3 = NEG_INF;
-        auto maxes = [&](uint32_t (&r)[32]) {
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            mx0 = fmaxf(mx0, __uint_as_float(r[j]));
-            mx1 = fmaxf(mx1, __uint_as_float(r[j + 1]));
-            mx2 = fmaxf(mx2, __uint_as_float(r[j + 2]));
-            mx3 = fmaxf(mx3, __uint_as_float(r[j + 3]));
+        for (int ch = 0; ch < 4; ++ch) {
+          tmem_wait_ld(r[ch]);
+          if (masked) mask(r[ch], 32 * ch);
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            mx0 = max3_nan(mx0, __uint_as_float(r[ch][j]), __uint_as_float(r[ch][j + 1]));
+            mx1 = max3_nan(mx1, __uint_as_float(r[ch][j + 2]), __uint_as_float(r[ch][j + 3]));
+            mx2 = max3_nan(mx2, __uint_as_float(r[ch][j + 4]), __uint_as_float(r[ch][j + 5]));
+            mx3 = max3_nan(mx3, __uint_as_float(r[ch][j + 6]), __uint_as_float(r[ch][j + 7]));
           }
-        };
-        tmem_ld32(tS, ra);
-#pragma unroll
-        for (int ch = 0; ch < 4; ch += 2) {
-          tmem_wait_ld(ra);
-          tmem_ld32(tS + 32 * (ch + 1), rb);
-          if (masked) mask(ra, 32 * ch);
-          maxes(ra);
-          tmem_wait_ld(rb);
-          if (ch == 0) tmem_ld32(tS + 64, ra);
-          if (masked) mask(rb, 32 * ch + 32);
-          maxes(rb);
         }
-        const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * c;
+        const float mx = max3_nan(max3_nan(mx0, mx1, mx2), mx3, mx3) * c;
         // The reference maximum moves only when a logit exceeds it by more than
         // LAZY (log2 units): any reference gives the same softmax once O and l
         // are normalised together, and O is rescaled in the first tiles only.
-        const bool grow = mx > m + LAZY;
+        // A NaN logit makes the reference, and so the whole row, NaN.
+        const bool grow = !(mx <= m + LAZY);
         if (__any_sync(0xffffffffu, grow)) {
           const float mn = grow ? mx : m;
           const float al = (m == NEG_INF) ? 0.f : ex2(m - mn);
@@ -323,39 +330,38 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
           m = mn;
         }
         const float mb = (m == NEG_INF ? 0.f : m) - BIAS;
-        // ---- P = 2^(x - m + BIAS), 32 columns at a time
-        tmem_ld32(tS, ra);
-        float l0 = 0.f, l1 = 0.f;
-        auto probs = [&](uint32_t (&r)[32], int ch) {
+        // ---- P = 2^(x - m + BIAS).  Special-function units give 16 exponentials
+        // a cycle and SM, as many as the tensor cores take; every third pair is
+        // computed on the FMA units instead.
+        const f2 c2 = mk2(c, c), mb2 = mk2(-mb, -mb);
+        f2 l0 = mk2(0.f, 0.f), l1 = mk2(0.f, 0.f);
+#pragma unroll
+        for (int ch = 0; ch < 4; ++ch) {
           uint32_t w[16];
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            const float p0 = ex2(fmaf(__uint_as_float(r[2 * j]), c, -mb));
-            const float p1 = ex2(fmaf(__uint_as_float(r[2 * j + 1]), c, -mb));
-            l0 += p0;
-            l1 += p1;
+            f2 x = fma2(mk2(__uint_as_float(r[ch][2 * j]), __uint_as_float(r[ch][2 * j + 1])), c2, mb2);
+            float p0, p1;
+            if (PSHARE > 0 && (16 * ch + j) % 8 < PSHARE) {
+              x = exp2_fma(x);
+              split2(x, p0, p1);
+            } else {
+              split2(x, p0, p1);
+              p0 = ex2(p0);
+              p1 = ex2(p1);
+              x = mk2(p0, p1);
+            }
+            if (j & 1) l1 = add2(l1, x);
+            else l0 = add2(l0, x);
             w[j] = pack2<MBF16>(p0, p1);
           }
           tmem_st16(tS + 16 * ch, w);
-        };
-#pragma unroll
-        for (int ch = 0; ch < 4; ch += 2) {
-          tmem_wait_ld(ra);
-          tmem_ld32(tS + 32 * (ch + 1), rb);
-          if (masked) mask(ra, 32 * ch);
-          if (ch == 0) {
-            // P of chunk 0 lands on S of chunk 0 only
-            probs(ra, 0);
-            tmem_wait_ld(rb);
-            tmem_ld32(tS + 64, ra);
-          } else {
-            probs(ra, 2);
-            tmem_wait_ld(rb);
-          }
-          if (masked) mask(rb, 32 * ch + 32);
-          probs(rb, ch + 1);
         }
-        l += l0 + l1;
+        {
+          float s0, s1;
+          split2(add2(l0, l1), s0, s1);
+          l += s0 + s1;
+        }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -390,6 +396,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
     }
   } else if (warp < 12) {
     // ============================================================ loaders
+    reg_dec<RLOAD>();
     const int lw = warp - 8, lt = tid - 256;
     int stage = 0;
     uint32_t eph = 1, qph = 1;
@@ -399,10 +406,6 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
     bool withhold = p.inject == 1;
     uint32_t raw_par = 0;  // parity of each raw slot's next completion
     uint32_t armed = 0, armed_par = 0;  // stages this warp has armed with copies, and the parity each was armed in
-    if (lane == 0) {
-      prefetch_tmap(&p.tk);
-      prefetch_tmap(&p.tv);
-    }
     // A tile's pages, one per lane (8 distinct), and whether a plain load of all
     // of them is right: every page in the pool, every token before the end.
     auto lookup = [&](int tile) -> int {
@@ -424,23 +427,25 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
       bool is_v;
       int tile = sg.t0 + load_item(0, sg.tiles, sg.dual, &is_v);
       int ent = lookup(tile);
-      // ---- Q: the unit's row tiles, once the previous segment's products are
-      // done; Q of the MMA's type with aligned rows is copied asynchronously
-      // while the first tile is requested
-      if (!(alive = wait(&b_qempty, qph))) break;
-      qph ^= 1u;
-      const bool q_async = p.q_al16 != 0 && p.q_dtype == (MBF16 ? FK_DTYPE_BF16 : FK_DTYPE_F16) && flip == 0;
-      {
-        constexpr int CPR = D / 8;  // 16-byte chunks of a row
+      // ---- Q: the unit's row tiles, behind the request of the first tile and
+      // once the previous segment's products are done
+      auto load_q = [&]() -> bool {
+        if (!wait(&b_qempty, qph)) return false;
+        qph ^= 1u;
+        // Q of the MMA's type with aligned rows is copied asynchronously
+        const bool q_async = p.q_al16 != 0 && p.q_dtype == (MBF16 ? FK_DTYPE_BF16 : FK_DTYPE_F16) && flip == 0;
+        constexpr int CPR = D / 8, RPS = 128 / CPR;  // 16-byte chunks of a row, rows of a step
         const int ch = lt % CPR;
+        const int db = RPS / p.G, dg = RPS - db * p.G;  // a step in sequences and group members
 #pragma unroll 1
         for (int s = 0; s < (sg.dual ? 2 : 1); ++s) {
           const uint32_t dst = sQ + s * C::TILE_BYTES + (ch >> 3) * HALF_BYTES;
+          int grow = (2 * sg.unit + s) * PROWS + lt / CPR;
+          int b = grow / p.G, gg = grow - b * p.G;
 #pragma unroll 8
-          for (int r = lt / CPR; r < PROWS; r += 128 / CPR) {
-            const int grow = (2 * sg.unit + s) * PROWS + r;
-            const int b = grow / p.G, gg = grow - b * p.G;
-            const long long e = b * p.q_b + static_cast<long long>(sg.h * p.G + gg) * p.q_h + ch * 8;
+          for (int k = 0; k < PROWS / RPS; ++k) {
+            const int r = lt / CPR + k * RPS;
+            const long long e = b * p.q_b + (sg.h * p.G + gg) * p.q_h + ch * 8;
             const uint32_t d = dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
             const bool in = grow < p.rows;
             if (q_async) {
@@ -449,15 +454,21 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
               const uint4 x = in ? load_q8<MBF16>(p, e, sq, flip) : make_uint4(0u, 0u, 0u, 0u);
               sts128(d, x.x, x.y, x.z, x.w);
             }
+            grow += RPS;
+            b += db;
+            gg += dg;
+            if (gg >= p.G) {
+              gg -= p.G;
+              ++b;
+            }
           }
         }
         cp_async_commit();
-      }
-      auto publish_q = [&]() {
         cp_async_wait<0>();
         fence_async_proxy();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&b_qfull));
+        return true;
       };
 
       // ---- K and V tiles
@@ -511,7 +522,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
             if (lane == 0) mbar_arrive(full);
           }
           advance();
-          if (idx == 0) publish_q();
+          if (idx == 0 && !(alive = load_q())) break;
         }
       } else {
         // e4m3: raw pages RAW - 1 tiles ahead; this warp widens its own 32 rows
@@ -546,7 +557,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
 #pragma unroll
         for (int i = 0; i < RAW - 1; ++i)
           if (req < items) request(i);
-        publish_q();
+        alive = load_q();
         for (int i0 = 0; i0 < items && alive; i0 += RAW) {
 #pragma unroll
           for (int sl = 0; sl < RAW; ++sl) {
@@ -613,51 +624,56 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
       }
     }
     if (s_bad && lane == 0 && p.status != nullptr) atomicOr(p.status, FK_STATUS_BAD_PAGE);
-  } else if (lane == 0) {
-    // ============================================================ MMA issue (one thread)
+  } else {
+    reg_dec<RMMA>();
+    if (warp == 12) {
+    // ============================================================ MMA issue (the whole warp walks, one lane issues)
     constexpr uint32_t idQK = instr_desc(MBF16, PROWS, PTOK, false);
     constexpr uint32_t idPV = instr_desc(MBF16, PROWS, D, true);
     int stage = 0;
     uint32_t fph = 0, qph = 0, pph[2] = {0, 0};
     bool alive = true;
-    auto wait1 = [&](uint64_t* bar, uint32_t parity) -> bool {
-      if (mbar_wait(smem_u32(bar), parity, p.wait_ns)) return true;
-      if (p.status != nullptr) atomicOr(p.status, FK_STATUS_TIMEOUT);
-      return false;
-    };
+    const bool leader = elect_one();
     // The tile at the head of the ring: waits for it on its first use, gives it
     // back after its last.
-    auto tile_in = [&]() -> bool { return wait1(&b_full[stage], fph); };
+    auto tile_in = [&]() -> bool { return wait(&b_full[stage], fph); };
     auto tile_out = [&]() {
-      mma_commit(smem_u32(&b_empty[stage]));
+      if (leader) mma_commit(smem_u32(&b_empty[stage]));
       if (++stage == ST) {
         stage = 0;
         fph ^= 1u;
       }
     };
+    // S = Q K^T of stream s: Q of row tile qt, K at k_addr
     auto qk = [&](int s, int qt, uint32_t k_addr) {
-      const uint32_t q_addr = sQ + qt * C::TILE_BYTES;
+      const uint32_t q_lo = desc_lo(sQ + qt * C::TILE_BYTES, 16), k_lo = desc_lo(k_addr, 16);
+      if (leader) {
+        mma_ss<false>(s * 128, q_lo, k_lo, idQK);
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        const uint32_t off = (k >> 2) * HALF_BYTES + (k & 3) * 32;
-        mma_ss(tmem + s * 128, smem_desc(q_addr + off, 16, 1024), smem_desc(k_addr + off, 16, 1024), idQK, k > 0);
+        for (int k = 1; k < D / 16; ++k) {
+          const uint32_t off = ((k >> 2) * HALF_BYTES + (k & 3) * 32) >> 4;
+          mma_ss<true>(s * 128, q_lo + off, k_lo + off, idQK);
+        }
+        mma_commit(smem_u32(&b_s[s]));
       }
-      mma_commit(smem_u32(&b_s[s]));
     };
+    // O (+)= P V of stream s
     auto pv = [&](int s, uint32_t v_addr, bool first) {
+      const uint32_t v_lo = desc_lo(v_addr, HALF_BYTES);
+      if (leader) {
 #pragma unroll
-      for (int k = 0; k < PTOK / 16; ++k)
-        mma_ts(tmem + 256 + s * D, tmem + s * 128 + 8 * k, smem_desc(v_addr + k * 2048, HALF_BYTES, 1024), idPV,
-               !first || k > 0);
+        for (int k = 0; k < PTOK / 16; ++k)
+          mma_ts(256 + s * D, s * 128 + 8 * k, v_lo + k * (2048 >> 4), idPV, !first || k > 0);
+      }
     };
     for (long long g = g0; g < g1 && alive;) {
       PrefixSeg sg;
       g += prefix_segment(pl, g, g1, blockIdx.x, &sg);
       const int n = sg.tiles;
-      if (!(alive = wait1(&b_qfull, qph))) break;
+      if (!(alive = wait(&b_qfull, qph))) break;
       qph ^= 1u;
       auto wait_p = [&](int s) -> bool {
-        if (!wait1(&b_p[s], pph[s])) return false;
+        if (!wait(&b_p[s], pph[s])) return false;
         pph[s] ^= 1u;
         tc_fence_after();
         return true;
@@ -678,10 +694,10 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
           if (!(alive = wait_p(0))) break;
           pv(0, v_addr, i == 0);
           if (i + 1 < n) {
-            if (!(alive = wait1(&b_full[ks], kph))) break;
+            if (!(alive = wait(&b_full[ks], kph))) break;
             qk(0, 0, k_addr);
           } else {
-            mma_commit(smem_u32(&b_o[0]));
+            if (leader) mma_commit(smem_u32(&b_o[0]));
           }
           if (!(alive = wait_p(1))) break;
           pv(1, v_addr, i == 0);
@@ -690,7 +706,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
             qk(1, 1, k_addr);
             tile_out();  // K_(i+1)
           } else {
-            mma_commit(smem_u32(&b_o[1]));
+            if (leader) mma_commit(smem_u32(&b_o[1]));
           }
         }
       } else {
@@ -710,22 +726,23 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
             qk(s, 0, sKV + stage * C::TILE_BYTES);
             tile_out();
           } else {
-            mma_commit(smem_u32(&b_o[s]));
+            if (leader) mma_commit(smem_u32(&b_o[s]));
           }
         }
       }
       if (!alive) break;
-      mma_commit(smem_u32(&b_qempty));
+      if (leader) mma_commit(smem_u32(&b_qempty));
     }
     // nothing of this thread's is in flight when the tensor memory is given back
-    mma_commit(smem_u32(&b_drain));
+    if (leader) mma_commit(smem_u32(&b_drain));
     mbar_wait(smem_u32(&b_drain), 0, p.wait_ns);
+    }
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 12) tmem_dealloc(tmem, 512);
+  if (warp == 12) tmem_dealloc(*const_cast<volatile uint32_t*>(&s_tmem), 512);
 }
 
 // ------------------------------------------------------------------------
@@ -830,8 +847,9 @@ __global__ void __launch_bounds__(JTHREADS) join_kernel(const __grid_constant__ 
   if (M == NEG_INF) e = 0.f, Lf = 0.f;  // nothing attended: zeros, whatever the sink
   else sink_norm(L, M, p.s_aux, qh, &e, &Lf);
   const float sv = p.scale_v != nullptr ? __ldg(p.scale_v) : 1.f;
-  const float o0 = norm_out(A.x, e, Lf, sv), o1 = norm_out(A.y, e, Lf, sv), o2 = norm_out(A.z, e, Lf, sv),
-              o3 = norm_out(A.w, e, Lf, sv);
+  const float f = Lf == 0.f ? 0.f : sv;  // a NaN stays one
+  const float o0 = f == 0.f ? 0.f : A.x * e / Lf * f, o1 = f == 0.f ? 0.f : A.y * e / Lf * f,
+              o2 = f == 0.f ? 0.f : A.z * e / Lf * f, o3 = f == 0.f ? 0.f : A.w * e / Lf * f;
   const long long ob = b * p.o_b + qh * p.o_h + d0;
   const bool bf = p.out_dtype == FK_DTYPE_BF16;
   if (p.o_al8) {

@@ -36,6 +36,7 @@
 #include <cstdint>
 
 #include "../../include/fk_decode.h"
+#include "fk_f32x2.cuh"
 #include "fk_host.h"
 #include "fk_prefix.h"
 #include "fk_ptx.cuh"
@@ -43,39 +44,6 @@
 namespace fk {
 
 constexpr int ROPE_THREADS = 128;
-
-// ---- packed f32 pairs
-struct f2 {
-  uint64_t v;
-};
-__device__ __forceinline__ f2 mk2(float lo, float hi) {
-  f2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ void split2(f2 a, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v));
-}
-__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
-  f2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
-  f2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-__device__ __forceinline__ f2 neg2(f2 a) {
-  float lo, hi;
-  split2(a, lo, hi);
-  return mk2(-lo, -hi);
-}
-__device__ __forceinline__ f2 swap2(f2 a) {
-  float lo, hi;
-  split2(a, lo, hi);
-  return mk2(hi, lo);
-}
 
 // Four 16-bit values <-> two pairs.
 template <bool BF>

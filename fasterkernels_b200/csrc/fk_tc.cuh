@@ -4,6 +4,8 @@
 
 #include <cstdint>
 
+#include "fk_f32x2.cuh"
+
 namespace fk {
 
 // ------------------------------------------------------------ tensor memory
@@ -71,14 +73,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
 
 // --------------------------------------------------------------- descriptors
 // Shared-memory operand, 128-byte swizzle (rows of 128 bytes, 16-byte chunk c
-// of row r at chunk c ^ (r & 7), 1024-byte aligned groups of 8 rows):
-//   K-major  (rows = M or N, columns = K): sbo = bytes between groups of 8 rows
-//   MN-major (rows = K, columns = M or N): sbo = bytes between groups of 8 rows,
-//            lbo = bytes between blocks of 64 columns
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-  return static_cast<uint64_t>((addr >> 4) & 0x3fffu) | (static_cast<uint64_t>(lbo >> 4) << 16) |
-         (static_cast<uint64_t>(sbo >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
+// of row r at chunk c ^ (r & 7), groups of 8 rows 1024 bytes apart):
+//   K-major  (rows = M or N, columns = K)
+//   MN-major (rows = K, columns = M or N): lbo = bytes between blocks of 64 columns
+// The upper word is the same for all of them; the lower one is advanced by
+// (byte offset >> 4) from one MMA to the next.
+constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) { return ((addr >> 4) & 0x3fffu) | ((lbo >> 4) << 16); }
 
 // Instruction descriptor of kind::f16 with f32 accumulation: A and B of one
 // type (bf16 or f16), A K-major, B K-major or MN-major.
@@ -87,21 +88,31 @@ __host__ __device__ constexpr uint32_t instr_desc(bool bf16, int m, int n, bool 
          (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-// One thread issues; D in tensor memory (+= when acc).
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+// One lane of the (converged) warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
+  return p != 0;
+}
+
+// One thread issues; D in tensor memory, += when ACC (or acc).  The operands
+// want to be warp-uniform: one held per thread is moved to a uniform register
+// before every MMA, which made the issuing thread the bottleneck.
+template <bool ACC>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc ? 1u : 0u)
+      "{\n .reg .pred p;\n .reg .b64 a, b;\n mov.b64 a, {%1, %3};\n mov.b64 b, {%2, %3};\n setp.ne.u32 p, %5, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n}\n" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(DESC_HI), "r"(idesc), "n"(ACC ? 1 : 0)
       : "memory");
 }
 
 // A (K-major, two 16-bit elements per column) in tensor memory.
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, bool acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc ? 1u : 0u)
+      "{\n .reg .pred p;\n .reg .b64 b;\n mov.b64 b, {%2, %3};\n setp.ne.u32 p, %5, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(DESC_HI), "r"(idesc), "r"(acc ? 1u : 0u)
       : "memory");
 }
 
@@ -128,6 +139,47 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Maximum of three, NaN if one is NaN.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
+// 2^x for x <= 127 without the special-function unit: x = n + f with n the
+// nearest integer (found by adding 1.5 * 2^23, whose low mantissa bits then
+// hold n), 2^f = 1 + f (c1 + f (c2 + f (c3 + f c4))) on [-1/2, 1/2], n added to
+// the exponent field.  The coefficients are the minimax fit of the relative
+// error (2.8e-6 = 2^-18.4, found by Lawson's iteration).  x below -125 gives
+// 2^-125.
+__device__ __forceinline__ f2 exp2_fma(f2 x) {
+  float lo, hi;
+  split2(x, lo, hi);
+  x = mk2(fmaxf(lo, -125.f), fmaxf(hi, -125.f));
+  const float big = 12582912.f;
+  const f2 t = add2(x, mk2(big, big));
+  const f2 f = fma2(add2(t, mk2(-big, -big)), mk2(-1.f, -1.f), x);
+  f2 p = fma2(f, mk2(0.009582852944731712f, 0.009582852944731712f), mk2(0.055906426161527634f, 0.055906426161527634f));
+  p = fma2(p, f, mk2(0.24024099111557007f, 0.24024099111557007f));
+  p = fma2(p, f, mk2(0.6931241750717163f, 0.6931241750717163f));
+  p = fma2(p, f, mk2(1.f, 1.f));
+  float plo, phi, tlo, thi;
+  split2(p, plo, phi);
+  split2(t, tlo, thi);
+  return mk2(__uint_as_float(__float_as_uint(plo) + (__float_as_uint(tlo) << 23)),
+             __uint_as_float(__float_as_uint(phi) + (__float_as_uint(thi) << 23)));
+}
+
+// Register share of a warpgroup from here on (all of its warps).
+template <int N>
+__device__ __forceinline__ void reg_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void reg_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 __device__ __forceinline__ void sts128(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
