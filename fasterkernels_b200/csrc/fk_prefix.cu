@@ -13,14 +13,16 @@
 // operations per KV head on 2 P D elements: tensor cores, not memory, carry it
 // from about 256 rows on.
 //
-//   tcgen05 tiles of 128 rows x 128 tokens; S (f32, 128 columns) and O (f32, D
-//   columns) live in tensor memory, two of each, so that two independent
-//   streams alternate: while one stream's softmax runs on the CUDA cores, the
-//   tensor cores work for the other.  With more than 128 rows the streams are
-//   two row tiles that share each K / V tile (dual); otherwise they are the
-//   even and the odd token tiles of one row tile (parity).
-//   P (f16, or bf16 for bf16 KV) overwrites the first half of its own S in
-//   tensor memory and is the A operand of O += P V from there.
+//   tcgen05 tiles of 128 rows x 64 tokens.  Two independent streams, each with
+//   a warpgroup of softmax threads (thread = row), take turns on the tensor
+//   cores; with more than 128 rows they are two row tiles that share each K / V
+//   tile (dual), otherwise the two halves of each token tile (parity).  Tensor
+//   memory holds for each stream O (f32, D columns) and two items of S (f32, 64
+//   columns each): S of item j + 1 is there before the softmax of item j ends,
+//   so that it never waits for the chain P V, Q K^T.  (With 128-token items there
+//   is room for one S a stream, and that chain, 1100 cycles, was added to every
+//   tile: 395 us for the long case below.)  P (f16, or bf16 for bf16 KV)
+//   overwrites half of its own S and is the A operand of O += P V from there.
 //
 // Work is cut like the decode kernel's: units (KV head, one or two row tiles)
 // laid end to end in granules (dual: one token tile, parity: two), each CTA of
@@ -28,8 +30,8 @@
 // CTA is a segment whose (max, sum, O) goes to the workspace.  Planned on the
 // device from the prefix length.
 //
-// Warps: 0-3 and 4-7 softmax of stream 0 and 1 (thread = row), 8-11 load Q, K
-// and V, 12 issues the MMAs.  A tile that the tensor cores read with one
+// Warps: 0-3 and 4-7 softmax of stream 0 and 1, 8-11 load Q, K and V, 12 issues
+// the MMAs.  A tile that the tensor cores read with one
 // descriptor needs its 8-row groups evenly spaced, so a page is loaded as one
 // box per 128-byte half, straight into its 16 rows of that half.  Each loader
 // warp loads two of a tile's eight pages: one warp issues a box in 100 to 150
@@ -50,15 +52,13 @@ namespace fk {
 #ifndef PSHARE
 #define PSHARE 3
 #endif
-#ifndef RSOFT
-#define RSOFT 184
-#define RLOAD 96
-#define RMMA 48
-#endif
+constexpr int SOFT_WARPS = 8;  // warps 0-7: softmax; 8-11 loaders; 12 MMA issue
+constexpr int LOAD_WARP = SOFT_WARPS, MMA_WARP = SOFT_WARPS + 4;
+constexpr int PTHREADS = (MMA_WARP + 1) * 32;
 constexpr int PROWS = 128;    // rows of a row tile (MMA M)
-constexpr int PTOK = 128;     // tokens of a token tile (MMA N of QK, K of PV)
+constexpr int PTOK = 128;     // tokens of a token tile (a K or V tile in shared memory)
+constexpr int PITEM = 64;     // tokens of an item (MMA N of QK, K of PV): half a tile
 constexpr int PPAGES = PTOK / PAGE;
-constexpr int PTHREADS = 16 * 32;  // four warpgroups (12-15: MMA issue, three idle warps)
 constexpr int HALF_BYTES = PTOK * 128;  // 128 rows of a 128-byte half
 
 template <int KV, int D>
@@ -68,8 +68,24 @@ struct PCfg {
   static constexpr int TILE_BYTES = NH * HALF_BYTES;  // Q, K or V tile in 16 bits
   static constexpr int STAGES = D == 64 ? 8 : FP8 ? 3 : 5;
   static constexpr int RAW = FP8 ? 4 : 0;             // e4m3 tiles on the way
-  static constexpr int SMEM = 1024 + (2 + STAGES) * TILE_BYTES + RAW * HALF_BYTES;
+  static constexpr int TILES = (2 + STAGES) * TILE_BYTES + RAW * HALF_BYTES;
 };
+
+// Barriers and small exchanges, behind the tiles.
+template <int ST, int RAW>
+struct PShared {
+  uint64_t full[ST], empty[ST], qfull, qempty, s[2][2], p[2][2], o[2], drain;
+  uint64_t raw[4][RAW];              // a loader warp's e4m3 pages
+  uint32_t tmem;
+  volatile int bad;                  // a bad page was seen: the softmax checks pages from then on
+};
+template <int KV, int D>
+constexpr int prefix_smem() {
+  using C = PCfg<KV, D>;
+  return C::TILES + static_cast<int>(sizeof(PShared<C::STAGES, C::RAW ? C::RAW : 1>));
+}
+static_assert(prefix_smem<FK_DTYPE_F16, 128>() <= 227 * 1024 && prefix_smem<FK_DTYPE_E4M3, 128>() <= 227 * 1024,
+              "shared memory of a block");
 
 struct PrefixParams {
   CUtensorMap tk, tv;  // boxes of one page's 16 rows x 128 bytes
@@ -93,40 +109,49 @@ struct PrefixParams {
   int inject;
 };
 
-// Granules and units, from the prefix length (device side).
+// Granules and units, from the prefix length (device side).  32-bit: the host
+// refuses more than 2^30 granules, and warps that gave their registers away
+// must not call the 64-bit division's slow path.
 struct PrefixPlan {
   int nt, nd, upu;       // token tiles; dual units and units of a KV head
-  long long gh, total, per;
+  int gh, total, per;    // granules of a KV head, in all, of a CTA
   __device__ PrefixPlan(int plen, int rows, int kv_heads, int ctas) {
     const int rt = (rows + PROWS - 1) / PROWS;
     nt = (plen + PTOK - 1) / PTOK;
     nd = rt / 2;
     upu = nd + (rt & 1);
-    gh = static_cast<long long>(nd) * nt + ((rt & 1) ? (nt + 1) / 2 : 0);
+    gh = nd * nt + ((rt & 1) ? (nt + 1) / 2 : 0);
     total = gh * kv_heads;
-    per = max((total + ctas - 1) / ctas, 1ll);
+    per = max((total + ctas - 1) / ctas, 1);
   }
   // First granule and length of unit u of a KV head.
-  __device__ long long unit_base(int u) const { return static_cast<long long>(u) * nt; }
+  __device__ int unit_base(int u) const { return u * nt; }
   __device__ int unit_len(int u) const { return u < nd ? nt : (nt + 1) / 2; }
 };
+
+// The prefix's length: at most what its table holds (tokens past that are
+// masked like those of a bad page).
+__device__ __forceinline__ int prefix_len(const int* dev, int host, int blocks, bool* past) {
+  const int n = max(dev != nullptr ? __ldg(dev) : host, 0);
+  *past = n > blocks * PAGE;
+  return min(n, blocks * PAGE);
+}
 
 struct PrefixSeg {
   int h, unit, seg, dual, t0, tiles;  // token tiles [t0, t0 + tiles)
 };
 
 // The segment at granule g of CTA c (granules [.., end)); returns its length.
-__device__ __forceinline__ long long prefix_segment(const PrefixPlan& pl, long long g, long long end, int c, PrefixSeg* s) {
-  s->h = static_cast<int>(g / pl.gh);
-  const long long r = g - s->h * pl.gh;
-  const long long dualg = static_cast<long long>(pl.nd) * pl.nt;
-  s->dual = r < dualg;
-  s->unit = s->dual ? static_cast<int>(r / pl.nt) : pl.nd;
-  const int off = static_cast<int>(r - pl.unit_base(s->unit));
-  const long long n = min(end - g, static_cast<long long>(pl.unit_len(s->unit) - off));
+__device__ __forceinline__ int prefix_segment(const PrefixPlan& pl, int g, int end, int c, PrefixSeg* s) {
+  s->h = g / pl.gh;
+  const int r = g - s->h * pl.gh;
+  s->dual = r < pl.nd * pl.nt;
+  s->unit = s->dual ? r / pl.nt : pl.nd;
+  const int off = r - pl.unit_base(s->unit);
+  const int n = min(end - g, pl.unit_len(s->unit) - off);
   s->seg = c + s->h * pl.upu + s->unit;
   s->t0 = s->dual ? off : 2 * off;
-  s->tiles = s->dual ? static_cast<int>(n) : static_cast<int>(min(2 * n, static_cast<long long>(pl.nt - 2 * off)));
+  s->tiles = s->dual ? n : min(2 * n, pl.nt - 2 * off);
   return n;
 }
 
@@ -193,37 +218,34 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
   // maximum's instead of 2^-25 (bf16 has f32's range and needs none).
   constexpr float BIAS = MBF16 ? 0.f : 7.f;
   constexpr float LAZY = 8.f;
-  extern __shared__ unsigned char smem_raw[];
-  const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t sQ = smem;                           // [2] row tiles
-  const uint32_t sKV = smem + 2 * C::TILE_BYTES;      // [ST]
+  extern __shared__ __align__(1024) unsigned char smem_raw[];  // 1024: the swizzle's period
+  const uint32_t sQ = smem_u32(smem_raw);             // [2] row tiles
+  const uint32_t sKV = sQ + 2 * C::TILE_BYTES;        // [ST]
   const uint32_t sRaw = sKV + ST * C::TILE_BYTES;     // [RAW][loader warp] two e4m3 pages
   constexpr int RAW = C::RAW > 0 ? C::RAW : 1;
-  __shared__ __align__(8) uint64_t b_raw[4][RAW];
-  __shared__ __align__(8) uint64_t b_full[ST], b_empty[ST], b_qfull, b_qempty, b_s[2], b_p[2], b_o[2], b_drain;
-  __shared__ uint32_t s_tmem;
-  __shared__ volatile int s_bad;  // a bad page was seen: the softmax checks pages from then on
+  PShared<ST, RAW>& sh = *reinterpret_cast<PShared<ST, RAW>*>(smem_raw + C::TILES);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
     for (int i = 0; i < ST; ++i) {
-      mbar_init(smem_u32(&b_full[i]), 4);
-      mbar_init(smem_u32(&b_empty[i]), 1);
+      mbar_init(smem_u32(&sh.full[i]), 4);
+      mbar_init(smem_u32(&sh.empty[i]), 1);
     }
-    mbar_init(smem_u32(&b_qfull), 4);
-    mbar_init(smem_u32(&b_qempty), 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_u32(&b_s[i]), 1);
-      mbar_init(smem_u32(&b_p[i]), 4);
-      mbar_init(smem_u32(&b_o[i]), 1);
+    mbar_init(smem_u32(&sh.qfull), 4);
+    mbar_init(smem_u32(&sh.qempty), 1);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(smem_u32(&sh.s[0][0] + i), 1);
+      mbar_init(smem_u32(&sh.p[0][0] + i), 4);
     }
-    mbar_init(smem_u32(&b_drain), 1);
-    for (int i = 0; i < 4 * RAW; ++i) mbar_init(smem_u32(&b_raw[0][0] + i), 1);
+    mbar_init(smem_u32(&sh.o[0]), 1);
+    mbar_init(smem_u32(&sh.o[1]), 1);
+    mbar_init(smem_u32(&sh.drain), 1);
+    for (int i = 0; i < 4 * RAW; ++i) mbar_init(smem_u32(&sh.raw[0][0] + i), 1);
     fence_mbar_init();
-    s_bad = 0;
+    sh.bad = 0;
   }
-  if (warp == 12) tmem_alloc(smem_u32(&s_tmem), 512);
-  if (tid == 8 * 32) {
+  if (warp == MMA_WARP) tmem_alloc(smem_u32(&sh.tmem), 512);
+  if (tid == LOAD_WARP * 32) {
     prefetch_tmap(&p.tk);
     prefetch_tmap(&p.tv);
   }
@@ -235,9 +257,11 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
   grid_dependency_trigger();
   for (int i = blockIdx.x * PTHREADS + tid; i < p.zero_words; i += gridDim.x * PTHREADS) p.zero[i] = 0;
 
-  const int plen = max(p.plen_dev != nullptr ? __ldg(p.plen_dev) : p.plen, 0);
+  bool past;
+  const int plen = prefix_len(p.plen_dev, p.plen, p.blocks, &past);
+  if (past && blockIdx.x == 0 && tid == 0 && p.status != nullptr) atomicOr(p.status, FK_STATUS_BAD_PAGE);
   const PrefixPlan pl(plen, p.rows, p.kv_heads, gridDim.x);
-  const long long g0 = blockIdx.x * pl.per, g1 = min(g0 + pl.per, pl.total);
+  const int g0 = min(static_cast<int>(blockIdx.x) * pl.per, pl.total), g1 = min(g0 + pl.per, pl.total);
   const float sk = (FP8 && p.scale_k != nullptr) ? __ldg(p.scale_k) : 1.f;
   auto timed_out = [&]() {
     if (lane == 0 && p.status != nullptr) atomicOr(p.status, FK_STATUS_TIMEOUT);
@@ -250,99 +274,102 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
     return false;
   };
 
-  if (warp < 8) {
+  if (warp < SOFT_WARPS) {
     // ============================================================ softmax
-    reg_inc<RSOFT>();
     const int s = warp >> 2;
-    const int row = tid & 127;
+    const int row = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // lane (warp & 3) * 32 in bits 16..
-    const uint32_t tS = tmem + lanes + s * 128, tO = tmem + lanes + 256 + s * D;
+    const uint32_t tO = tmem + lanes + 256 + s * D;
     // never 0: a masked logit (-inf) stays one
     const float c = fmaxf(rsqrtf(static_cast<float>(D)) * LOG2E * fabsf(sk), 1e-30f);
-    uint32_t sph = 0, oph = 0;
+    uint32_t sph = 0;  // parities of the two S buffers
+    uint32_t oph = 0;  // parity of the next P V
     bool alive = true;
-    for (long long g = g0; g < g1 && alive;) {
+    for (int g = g0; g < g1 && alive;) {
       PrefixSeg sg;
       g += prefix_segment(pl, g, g1, blockIdx.x, &sg);
-      const int n = sg.dual ? sg.tiles : (sg.tiles + 1 - s) / 2;  // token tiles of this stream
+      const int ni = sg.dual ? 2 * sg.tiles : sg.tiles;
       const int trow = (2 * sg.unit + (sg.dual ? s : 0)) * PROWS + row;
+      const int tok00 = sg.t0 * PTOK + (sg.dual ? 0 : s * PITEM), tstep = sg.dual ? PITEM : PTOK;
       float m = NEG_INF, l = 0.f;
-      for (int i = 0; i < n; ++i) {
-        const int tile = sg.t0 + (sg.dual ? i : 2 * i + s);
-        if (!(alive = wait(&b_s[s], sph))) break;
-        sph ^= 1u;
+      for (int j = 0; j < ni; ++j) {
+        const int buf = j & 1;
+        const int tok0 = tok00 + j * tstep;  // the item's first token
+        const uint32_t tS = tmem + lanes + s * 128 + buf * PITEM;
+        if (!(alive = wait(&sh.s[s][buf], (sph >> buf) & 1u))) break;
+        sph ^= 1u << buf;
         tc_fence_after();
-        const int lim = plen - tile * PTOK;  // tokens of the tile that exist
-        uint32_t okp = 0xffu;                // its pages that do
-        if (s_bad) {
+        // ---- the row of S, its maximum
+        uint32_t r[2][32];
+        tmem_ld32(tS, r[0]);
+        tmem_ld32(tS + 32, r[1]);
+        const int lim = plen - tok0;  // tokens of the item that exist
+        uint32_t okp = 0xfu;          // its pages that do
+        if (sh.bad) {
           okp = 0;
-          for (int j = 0; j < PPAGES; ++j) {
-            const int pg = tile * PPAGES + j;
+          for (int k = 0; k < PITEM / PAGE; ++k) {
+            const int pg = tok0 / PAGE + k;
             const int ph = pg < p.blocks ? __ldg(p.table + pg) : -1;
-            okp |= (ph >= 0 && ph < p.num_pages ? 1u : 0u) << j;
+            okp |= (ph >= 0 && ph < p.num_pages ? 1u : 0u) << k;
           }
         }
-        const bool masked = lim < PTOK || okp != 0xffu;
-        auto mask = [&](uint32_t (&r)[32], int col) {
+        tmem_wait_ld(r[0]);
+        tmem_wait_ld(r[1]);
+        if (lim < PITEM || okp != 0xfu) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (col + j >= lim || !((okp >> ((col + j) >> 4)) & 1u)) r[j] = __float_as_uint(NEG_INF);
-        };
-        // ---- the row of S, its maximum
-        uint32_t r[4][32];
-#pragma unroll
-        for (int ch = 0; ch < 4; ++ch) tmem_ld32(tS + 32 * ch, r[ch]);
+          for (int k = 0; k < PITEM; ++k)
+            if (k >= lim || !((okp >> (k >> 4)) & 1u)) r[k >> 5][k & 31] = __float_as_uint(NEG_INF);
+        }
         float mx0 = NEG_INF, mx1 = NEG_INF, mx2 = NEG_INF, mx3 = NEG_INF;
 #pragma unroll
-        for (int ch = 0; ch < 4; ++ch) {
-          tmem_wait_ld(r[ch]);
-          if (masked) mask(r[ch], 32 * ch);
-#pragma unroll
-          for (int j = 0; j < 32; j += 8) {
-            mx0 = max3_nan(mx0, __uint_as_float(r[ch][j]), __uint_as_float(r[ch][j + 1]));
-            mx1 = max3_nan(mx1, __uint_as_float(r[ch][j + 2]), __uint_as_float(r[ch][j + 3]));
-            mx2 = max3_nan(mx2, __uint_as_float(r[ch][j + 4]), __uint_as_float(r[ch][j + 5]));
-            mx3 = max3_nan(mx3, __uint_as_float(r[ch][j + 6]), __uint_as_float(r[ch][j + 7]));
-          }
+        for (int k = 0; k < PITEM; k += 8) {
+          const uint32_t* q = &r[k >> 5][k & 31];
+          mx0 = max3_nan(mx0, __uint_as_float(q[0]), __uint_as_float(q[1]));
+          mx1 = max3_nan(mx1, __uint_as_float(q[2]), __uint_as_float(q[3]));
+          mx2 = max3_nan(mx2, __uint_as_float(q[4]), __uint_as_float(q[5]));
+          mx3 = max3_nan(mx3, __uint_as_float(q[6]), __uint_as_float(q[7]));
         }
         const float mx = max3_nan(max3_nan(mx0, mx1, mx2), mx3, mx3) * c;
         // The reference maximum moves only when a logit exceeds it by more than
         // LAZY (log2 units): any reference gives the same softmax once O and l
-        // are normalised together, and O is rescaled in the first tiles only.
+        // are normalised together, and O is rescaled in the first items only.
         // A NaN logit makes the reference, and so the whole row, NaN.
         const bool grow = !(mx <= m + LAZY);
         if (__any_sync(0xffffffffu, grow)) {
           const float mn = grow ? mx : m;
           const float al = (m == NEG_INF) ? 0.f : ex2(m - mn);
           l *= al;
-          if (i > 0) {
-            // S of this tile is complete, hence so is every earlier P V of this stream
-            uint32_t o[32];
+          if (j > 0) {
+            // the previous item's P V (S of this item says that the one before
+            // it is complete)
+            if (!(alive = wait(&sh.o[s], oph ^ 1u))) break;
+            tc_fence_after();
+            uint32_t o[16];
 #pragma unroll 1
-            for (int d = 0; d < D; d += 32) {
-              tmem_ld32(tO + d, o);
+            for (int d = 0; d < D; d += 16) {
+              tmem_ld16(tO + d, o);
               tmem_wait_ld(o);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * al);
-              tmem_st32(tO + d, o);
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * al);
+              tmem_st16(tO + d, o);
             }
           }
           m = mn;
         }
         const float mb = (m == NEG_INF ? 0.f : m) - BIAS;
         // ---- P = 2^(x - m + BIAS).  Special-function units give 16 exponentials
-        // a cycle and SM, as many as the tensor cores take; every third pair is
+        // a cycle and SM, as many as the tensor cores take; some pairs are
         // computed on the FMA units instead.
         const f2 c2 = mk2(c, c), mb2 = mk2(-mb, -mb);
         f2 l0 = mk2(0.f, 0.f), l1 = mk2(0.f, 0.f);
 #pragma unroll
-        for (int ch = 0; ch < 4; ++ch) {
+        for (int ch = 0; ch < 2; ++ch) {
           uint32_t w[16];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            f2 x = fma2(mk2(__uint_as_float(r[ch][2 * j]), __uint_as_float(r[ch][2 * j + 1])), c2, mb2);
+          for (int k = 0; k < 16; ++k) {
+            f2 x = fma2(mk2(__uint_as_float(r[ch][2 * k]), __uint_as_float(r[ch][2 * k + 1])), c2, mb2);
             float p0, p1;
-            if (PSHARE > 0 && (16 * ch + j) % 8 < PSHARE) {
+            if (PSHARE > 0 && k % 8 < PSHARE) {
               x = exp2_fma(x);
               split2(x, p0, p1);
             } else {
@@ -351,11 +378,11 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
               p1 = ex2(p1);
               x = mk2(p0, p1);
             }
-            if (j & 1) l1 = add2(l1, x);
+            if (k & 1) l1 = add2(l1, x);
             else l0 = add2(l0, x);
-            w[j] = pack2<MBF16>(p0, p1);
+            w[k] = pack2<MBF16>(p0, p1);
           }
-          tmem_st16(tS + 16 * ch, w);
+          tmem_st16(tS + 16 * ch, w);  // over S, which is in registers
         }
         {
           float s0, s1;
@@ -365,39 +392,37 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&b_p[s]));
+        if (lane == 0) mbar_arrive(smem_u32(&sh.p[s][buf]));
+        oph ^= 1u;
       }
       if (!alive) break;
-      const long long rec = (static_cast<long long>(sg.seg) * 2 + s);
-      if (n > 0) {
-        if (!(alive = wait(&b_o[s], oph))) break;
-        oph ^= 1u;
-        tc_fence_after();
-      }
+      const long long rec = static_cast<long long>(sg.seg) * 2 + s;
+      // The last P V.  S of the last item only says that the third last P V is
+      // complete, and a parity tells two neighbouring ones apart: one at a time.
+      if (ni > 1 && !(alive = wait(&sh.o[s], oph))) break;
+      if (!(alive = wait(&sh.o[s], oph ^ 1u))) break;
+      tc_fence_after();
       const bool valid = trow < p.rows;
       if (valid) p.ml[rec * PROWS + row] = make_float2(m == NEG_INF ? NEG_INF : m - BIAS, l);
-      if (n > 0) {
-        // [D / 4][128 rows][4]: a warp stores 512 contiguous bytes
-        float4* dst = reinterpret_cast<float4*>(p.acc + rec * PROWS * D) + row;
+      // [D / 4][128 rows][4]: a warp stores 512 contiguous bytes
+      float4* dst = reinterpret_cast<float4*>(p.acc + rec * PROWS * D) + row;
 #pragma unroll 1
-        for (int d = 0; d < D; d += 32) {
-          uint32_t o[32];
-          tmem_ld32(tO + d, o);
-          tmem_wait_ld(o);
-          if (valid) {
+      for (int d = 0; d < D; d += 32) {
+        uint32_t o[32];
+        tmem_ld32(tO + d, o);
+        tmem_wait_ld(o);
+        if (valid) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              dst[(d / 4 + j) * PROWS] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]),
-                                                     __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
-          }
+          for (int k = 0; k < 8; ++k)
+            dst[(d / 4 + k) * PROWS] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]),
+                                                   __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
         }
-        tc_fence_before();
       }
+      tc_fence_before();
     }
-  } else if (warp < 12) {
+  } else if (warp < LOAD_WARP + 4) {
     // ============================================================ loaders
-    reg_dec<RLOAD>();
-    const int lw = warp - 8, lt = tid - 256;
+    const int lw = warp - LOAD_WARP, lt = tid - LOAD_WARP * 32;
     int stage = 0;
     uint32_t eph = 1, qph = 1;
     const float sq = p.scale_q != nullptr ? __ldg(p.scale_q) : 1.f;
@@ -420,7 +445,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
         eph ^= 1u;
       }
     };
-    for (long long g = g0; g < g1 && alive;) {
+    for (int g = g0; g < g1 && alive;) {
       PrefixSeg sg;
       g += prefix_segment(pl, g, g1, blockIdx.x, &sg);
       const int items = 2 * sg.tiles;
@@ -430,7 +455,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
       // ---- Q: the unit's row tiles, behind the request of the first tile and
       // once the previous segment's products are done
       auto load_q = [&]() -> bool {
-        if (!wait(&b_qempty, qph)) return false;
+        if (!wait(&sh.qempty, qph)) return false;
         qph ^= 1u;
         // Q of the MMA's type with aligned rows is copied asynchronously
         const bool q_async = p.q_al16 != 0 && p.q_dtype == (MBF16 ? FK_DTYPE_BF16 : FK_DTYPE_F16) && flip == 0;
@@ -467,7 +492,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
         cp_async_wait<0>();
         fence_async_proxy();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&b_qfull));
+        if (lane == 0) mbar_arrive(smem_u32(&sh.qfull));
         return true;
       };
 
@@ -480,8 +505,8 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
             tile = sg.t0 + load_item(idx + 1, sg.tiles, sg.dual, &is_v);
             ent = lookup(tile);
           }
-          if (!(alive = wait(&b_empty[stage], eph))) break;
-          const uint32_t full = smem_u32(&b_full[stage]);
+          if (!(alive = wait(&sh.empty[stage], eph))) break;
+          const uint32_t full = smem_u32(&sh.full[stage]);
           const uint32_t dst = sKV + stage * C::TILE_BYTES;
           const bool all = plain(t, e);
           const int ph0 = __shfl_sync(0xffffffffu, e, 2 * lw), ph1 = __shfl_sync(0xffffffffu, e, 2 * lw + 1);
@@ -510,7 +535,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
               const int r = u / CPR, ch = u % CPR, tok = t * PTOK + 32 * lw + r;
               const int ph = r < 16 ? ph0 : ph1;
               const bool ok = ph >= 0 && tok < plen;
-              if (ph < 0 && tok < plen) s_bad = 1;
+              if (ph < 0 && tok < plen) sh.bad = 1;
               const int row = 32 * lw + r;
               cp_async16_zfill(dst + (ch >> 3) * HALF_BYTES + row * 128 + (((ch & 7) ^ (row & 7)) << 4),
                                ok ? base + ph * sp + (r & 15) * ss + ch * 16 : base, ok);
@@ -544,7 +569,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
           qph1[slot] = __shfl_sync(0xffffffffu, rent, 2 * lw + 1);
           if (qall[slot] && lane == 0) {
             const CUtensorMap* map = rv ? &p.tv : &p.tk;
-            const uint32_t bar = smem_u32(&b_raw[lw][slot]);
+            const uint32_t bar = smem_u32(&sh.raw[lw][slot]);
             mbar_arrive_expect_tx(bar, 4096);
             tma_load_4d(raw0 + slot * HALF_BYTES, map, bar, 0, 0, sg.h, qph0[slot]);
             tma_load_4d(raw0 + slot * HALF_BYTES + 2048, map, bar, 0, 0, sg.h, qph1[slot]);
@@ -570,7 +595,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
             const int ch = lane & 7, r0 = lane >> 3;
             uint4 x[8];
             if (qall[sl]) {
-              if (!(alive = wait(&b_raw[lw][sl], (raw_par >> sl) & 1u))) break;
+              if (!(alive = wait(&sh.raw[lw][sl], (raw_par >> sl) & 1u))) break;
               raw_par ^= 1u << sl;
 #pragma unroll
               for (int k = 0; k < 8; ++k) {
@@ -584,12 +609,12 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
               for (int k = 0; k < 8; ++k) {
                 const int r = r0 + 4 * k, tok = t * PTOK + 32 * lw + r;
                 const int ph = r < 16 ? ph0 : ph1;
-                if (ph < 0 && tok < plen) s_bad = 1;
+                if (ph < 0 && tok < plen) sh.bad = 1;
                 x[k] = make_uint4(0u, 0u, 0u, 0u);
                 if (ph >= 0 && tok < plen) x[k] = __ldg(reinterpret_cast<const uint4*>(base + ph * sp + (r & 15) * ss + ch * 16));
               }
             }
-            if (!(alive = wait(&b_empty[stage], eph))) break;
+            if (!(alive = wait(&sh.empty[stage], eph))) break;
             const uint32_t dst = sKV + stage * C::TILE_BYTES + (ch >> 2) * HALF_BYTES + 32 * lw * 128;
             const int c0 = (2 * ch) & 7;
 #pragma unroll
@@ -606,7 +631,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
             // also orders the reads of the raw slot before its next copy
             fence_async_proxy();
             __syncwarp();
-            if (lane == 0 && !withhold) mbar_arrive(smem_u32(&b_full[stage]));
+            if (lane == 0 && !withhold) mbar_arrive(smem_u32(&sh.full[stage]));
             withhold = false;
             advance();
           }
@@ -617,132 +642,115 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
     cp_async_wait<0>();
     if (!alive && lane == 0) {
       if constexpr (FP8) {
-        for (int i = 0; i < RAW; ++i) mbar_wait(smem_u32(&b_raw[lw][i]), (raw_par >> i) & 1u, p.wait_ns);
+        for (int i = 0; i < RAW; ++i) mbar_wait(smem_u32(&sh.raw[lw][i]), (raw_par >> i) & 1u, p.wait_ns);
       } else {
         for (int i = 0; i < ST; ++i)
-          if ((armed >> i) & 1u) mbar_wait(smem_u32(&b_full[i]), (armed_par >> i) & 1u, p.wait_ns);
+          if ((armed >> i) & 1u) mbar_wait(smem_u32(&sh.full[i]), (armed_par >> i) & 1u, p.wait_ns);
       }
     }
-    if (s_bad && lane == 0 && p.status != nullptr) atomicOr(p.status, FK_STATUS_BAD_PAGE);
+    if (sh.bad && lane == 0 && p.status != nullptr) atomicOr(p.status, FK_STATUS_BAD_PAGE);
   } else {
-    reg_dec<RMMA>();
-    if (warp == 12) {
     // ============================================================ MMA issue (the whole warp walks, one lane issues)
-    constexpr uint32_t idQK = instr_desc(MBF16, PROWS, PTOK, false);
+    constexpr uint32_t idQK = instr_desc(MBF16, PROWS, PITEM, false);
     constexpr uint32_t idPV = instr_desc(MBF16, PROWS, D, true);
     int stage = 0;
-    uint32_t fph = 0, qph = 0, pph[2] = {0, 0};
+    uint32_t fph = 0, qph = 0, pph[2] = {0, 0};  // pph[s]: parities of the stream's two P buffers
     bool alive = true;
     const bool leader = elect_one();
-    // The tile at the head of the ring: waits for it on its first use, gives it
-    // back after its last.
-    auto tile_in = [&]() -> bool { return wait(&b_full[stage], fph); };
-    auto tile_out = [&]() {
-      if (leader) mma_commit(smem_u32(&b_empty[stage]));
-      if (++stage == ST) {
-        stage = 0;
-        fph ^= 1u;
-      }
-    };
-    // S = Q K^T of stream s: Q of row tile qt, K at k_addr
-    auto qk = [&](int s, int qt, uint32_t k_addr) {
+    // S = Q K^T of stream s, item buffer buf: Q of row tile qt, 64 rows of K at k_addr
+    auto qk = [&](int s, int buf, int qt, uint32_t k_addr) {
       const uint32_t q_lo = desc_lo(sQ + qt * C::TILE_BYTES, 16), k_lo = desc_lo(k_addr, 16);
       if (leader) {
-        mma_ss<false>(s * 128, q_lo, k_lo, idQK);
+        mma_ss<false>(s * 128 + buf * PITEM, q_lo, k_lo, idQK);
 #pragma unroll
         for (int k = 1; k < D / 16; ++k) {
           const uint32_t off = ((k >> 2) * HALF_BYTES + (k & 3) * 32) >> 4;
-          mma_ss<true>(s * 128, q_lo + off, k_lo + off, idQK);
+          mma_ss<true>(s * 128 + buf * PITEM, q_lo + off, k_lo + off, idQK);
         }
-        mma_commit(smem_u32(&b_s[s]));
+        mma_commit(smem_u32(&sh.s[s][buf]));
       }
     };
-    // O (+)= P V of stream s
-    auto pv = [&](int s, uint32_t v_addr, bool first) {
+    // O (+)= P V of stream s, item buffer buf: 64 rows of V at v_addr
+    auto pv = [&](int s, int buf, uint32_t v_addr, bool first) {
       const uint32_t v_lo = desc_lo(v_addr, HALF_BYTES);
       if (leader) {
 #pragma unroll
-        for (int k = 0; k < PTOK / 16; ++k)
-          mma_ts(256 + s * D, s * 128 + 8 * k, v_lo + k * (2048 >> 4), idPV, !first || k > 0);
+        for (int k = 0; k < PITEM / 16; ++k)
+          mma_ts(256 + s * D, s * 128 + buf * PITEM + 8 * k, v_lo + k * (2048 >> 4), idPV, !first || k > 0);
+        mma_commit(smem_u32(&sh.o[s]));
       }
     };
-    for (long long g = g0; g < g1 && alive;) {
+    for (int g = g0; g < g1 && alive;) {
       PrefixSeg sg;
       g += prefix_segment(pl, g, g1, blockIdx.x, &sg);
-      const int n = sg.tiles;
-      if (!(alive = wait(&b_qfull, qph))) break;
+      const bool dual = sg.dual;
+      const int ni = dual ? 2 * sg.tiles : sg.tiles;
+      // Item j of stream s: dual, 64-token half j & 1 of token tile j / 2;
+      // parity, half s of token tile j.
+      auto half_of = [&](int s, int j) -> uint32_t { return (dual ? (j & 1) : s) * (PITEM * 128); };
+      if (!(alive = wait(&sh.qfull, qph))) break;
       qph ^= 1u;
-      auto wait_p = [&](int s) -> bool {
-        if (!wait(&b_p[s], pph[s])) return false;
-        pph[s] ^= 1u;
-        tc_fence_after();
-        return true;
+      auto give_back = [&](int st) {
+        if (leader) mma_commit(smem_u32(&sh.empty[st]));
       };
-      if (sg.dual) {
-        // K0: both streams
-        if (!(alive = tile_in())) break;
-        qk(0, 0, sKV + stage * C::TILE_BYTES);
-        qk(1, 1, sKV + stage * C::TILE_BYTES);
-        tile_out();
-        for (int i = 0; i < n; ++i) {
-          // ring: V_i at the head, K_(i+1) behind it
-          if (!(alive = tile_in())) break;
-          const uint32_t v_addr = sKV + stage * C::TILE_BYTES;
-          const int ks = stage + 1 == ST ? 0 : stage + 1;
-          const uint32_t kph = stage + 1 == ST ? fph ^ 1u : fph;
-          const uint32_t k_addr = sKV + ks * C::TILE_BYTES;
-          if (!(alive = wait_p(0))) break;
-          pv(0, v_addr, i == 0);
-          if (i + 1 < n) {
-            if (!(alive = wait(&b_full[ks], kph))) break;
-            qk(0, 0, k_addr);
-          } else {
-            if (leader) mma_commit(smem_u32(&b_o[0]));
-          }
-          if (!(alive = wait_p(1))) break;
-          pv(1, v_addr, i == 0);
-          tile_out();  // V_i
-          if (i + 1 < n) {
-            qk(1, 1, k_addr);
-            tile_out();  // K_(i+1)
-          } else {
-            if (leader) mma_commit(smem_u32(&b_o[1]));
+      auto advance = [&]() {
+        if (++stage == ST) {
+          stage = 0;
+          fph ^= 1u;
+        }
+      };
+      // two items of S ahead of the softmax
+      for (int j = 0; j < min(ni, 2) && alive; ++j) {
+        if (!dual || j == 0) alive = wait(&sh.full[stage], fph);
+        if (!alive) break;
+        const uint32_t k_addr = sKV + stage * C::TILE_BYTES;
+        qk(0, j, 0, k_addr + half_of(0, j));
+        qk(1, j, dual ? 1 : 0, k_addr + half_of(1, j));
+        if (!dual || j == 1) {
+          give_back(stage);
+          advance();
+        }
+      }
+      // step j: P V of item j, S of item j + 2; the ring holds V at its head and
+      // K behind it (for two steps with dual)
+      for (int j = 0; j < ni && alive; ++j) {
+        const int buf = j & 1;
+        const bool first_use = !dual || buf == 0, last_use = !dual || buf == 1, more = j + 2 < ni;
+        if (first_use && !(alive = wait(&sh.full[stage], fph))) break;
+        const int ks = stage + 1 == ST ? 0 : stage + 1;
+        const uint32_t kph = stage + 1 == ST ? fph ^ 1u : fph;
+        const uint32_t v_addr = sKV + stage * C::TILE_BYTES, k_addr = sKV + ks * C::TILE_BYTES;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          if (!(alive = wait(&sh.p[s][buf], (pph[s] >> buf) & 1u))) break;
+          pph[s] ^= 1u << buf;
+          tc_fence_after();
+          pv(s, buf, v_addr + half_of(s, j), j == 0);
+          if (s == 1 && last_use) give_back(stage);
+          if (more) {
+            if (s == 0 && first_use && !(alive = wait(&sh.full[ks], kph))) break;
+            qk(s, buf, dual ? s : 0, k_addr + half_of(s, j));
+            if (s == 1 && last_use) give_back(ks);
           }
         }
-      } else {
-        const int pre = min(n, 2);
-        for (int s = 0; s < pre && alive; ++s) {
-          if (!(alive = tile_in())) break;
-          qk(s, 0, sKV + stage * C::TILE_BYTES);
-          tile_out();
-        }
-        for (int i = 0; i < n && alive; ++i) {
-          const int s = i & 1;
-          if (!(alive = tile_in()) || !(alive = wait_p(s))) break;
-          pv(s, sKV + stage * C::TILE_BYTES, i < 2);
-          tile_out();
-          if (i + 2 < n) {
-            if (!(alive = tile_in())) break;
-            qk(s, 0, sKV + stage * C::TILE_BYTES);
-            tile_out();
-          } else {
-            if (leader) mma_commit(smem_u32(&b_o[s]));
-          }
+        if (!alive) break;
+        if (last_use) {
+          advance();
+          if (more) advance();
         }
       }
       if (!alive) break;
-      if (leader) mma_commit(smem_u32(&b_qempty));
+      if (leader) mma_commit(smem_u32(&sh.qempty));
     }
-    // nothing of this thread's is in flight when the tensor memory is given back
-    if (leader) mma_commit(smem_u32(&b_drain));
-    mbar_wait(smem_u32(&b_drain), 0, p.wait_ns);
-    }
+    // nothing of this warp's is in flight when the tensor memory is given back
+    if (leader) mma_commit(smem_u32(&sh.drain));
+    mbar_wait(smem_u32(&sh.drain), 0, p.wait_ns);
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 12) tmem_dealloc(*const_cast<volatile uint32_t*>(&s_tmem), 512);
+  if (warp == MMA_WARP) tmem_dealloc(*const_cast<volatile uint32_t*>(&sh.tmem), 512);
 }
 
 // ------------------------------------------------------------------------
@@ -758,7 +766,7 @@ struct JoinParams {
   const float2* own_ml;   // [B, QH]
   const float* own_acc;   // [B, QH, D]
   const int* plen_dev;
-  int plen, rows, G, kv_heads, q_heads, ctas;
+  int plen, blocks, rows, G, kv_heads, q_heads, ctas;
   const float* s_aux;
   const float* scale_v;
   void* out;
@@ -788,17 +796,18 @@ __global__ void __launch_bounds__(JTHREADS) join_kernel(const __grid_constant__ 
   const long long orow = static_cast<long long>(b) * p.q_heads + qh;
   const float2 own = __ldcg(p.own_ml + orow);
   const float4 own_a = __ldcg(reinterpret_cast<const float4*>(p.own_acc + orow * D + d0));
-  const int plen = max(p.plen_dev != nullptr ? __ldg(p.plen_dev) : p.plen, 0);
+  bool past;
+  const int plen = prefix_len(p.plen_dev, p.plen, p.blocks, &past);
   const PrefixPlan pl(plen, p.rows, p.kv_heads, p.ctas);
   const int unit = tile >> 1;
   const bool dual = unit < pl.nd;
   long long rec0 = 0;  // the row's records: every (dual) second one from rec0 on
   int nrec = 0;
   if (pl.nt > 0) {
-    const long long base = h * pl.gh + pl.unit_base(unit);
-    const long long c0 = base / pl.per, c1 = (base + pl.unit_len(unit) - 1) / pl.per;
-    rec0 = 2 * (c0 + h * pl.upu + unit) + (dual ? (tile & 1) : 0);
-    nrec = static_cast<int>(c1 - c0 + 1) * (dual ? 1 : 2);
+    const int base = h * pl.gh + pl.unit_base(unit);
+    const int c0 = base / pl.per, c1 = (base + pl.unit_len(unit) - 1) / pl.per;
+    rec0 = 2ll * (c0 + h * pl.upu + unit) + (dual ? (tile & 1) : 0);
+    nrec = (c1 - c0 + 1) * (dual ? 1 : 2);
   }
   const int rstep = dual ? 2 : 1;
 
@@ -901,12 +910,12 @@ int launch_prefix(const PrefixParams& p, int ctas, int device, cudaStream_t stre
   {
     std::lock_guard<std::mutex> lk(mu);
     if (!done[device]) {
-      const cudaError_t e = cudaFuncSetAttribute(prefix_kernel<KV, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, PCfg<KV, D>::SMEM);
+      const cudaError_t e = cudaFuncSetAttribute(prefix_kernel<KV, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, prefix_smem<KV, D>());
       if (e != cudaSuccess) return fail(FK_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
       done[device] = true;
     }
   }
-  const cudaError_t e = launch_pdl(prefix_kernel<KV, D>, dim3(ctas), dim3(PTHREADS), PCfg<KV, D>::SMEM, stream, p);
+  const cudaError_t e = launch_pdl(prefix_kernel<KV, D>, dim3(ctas), dim3(PTHREADS), prefix_smem<KV, D>(), stream, p);
   return e == cudaSuccess ? FK_OK : fail(FK_ERR_CUDA, "prefix launch failed: %s", cudaGetErrorString(e));
 }
 
@@ -934,6 +943,13 @@ extern "C" int fk_paged_shared_prefix_decode(const fk_prefix_args* a, void* work
   if (a->num_pages <= 0 || a->num_pages > 0x7fffffffLL || a->max_blocks < 0 || a->max_blocks > 0x7fffffffLL ||
       a->prefix_blocks < 0 || a->prefix_blocks > 0x7ffffffLL || a->prefix_len < 0 || a->prefix_len > 0x7fffff00LL)
     return fail(FK_ERR_INVALID_ARG, "bad page counts or prefix length");
+  {
+    // granules of the prefix part (see PrefixPlan), and the CTAs added to them
+    const long long rt = (a->batch * (a->q_heads / a->kv_heads) + PROWS - 1) / PROWS, nt = (a->prefix_blocks * PAGE + PTOK - 1) / PTOK;
+    if (a->q_heads % a->kv_heads == 0 && a->kv_heads * ((rt + 1) / 2) * nt > (1ll << 30))
+      return fail(FK_ERR_UNSUPPORTED, "too many row tiles x prefix pages (%lld x %lld)", static_cast<long long>(a->kv_heads * rt),
+                  static_cast<long long>(a->prefix_blocks));
+  }
   if (a->prefix_table == nullptr && a->prefix_blocks > 0) return fail(FK_ERR_INVALID_ARG, "prefix_table must be non-null");
   OwnPart own;
   int device = 0;
@@ -1011,6 +1027,7 @@ extern "C" int fk_paged_shared_prefix_decode(const fk_prefix_args* a, void* work
   j.own_acc = reinterpret_cast<const float*>(ws + w.own_acc);
   j.plen_dev = p.plen_dev;
   j.plen = p.plen;
+  j.blocks = p.blocks;
   j.rows = p.rows;
   j.G = p.G;
   j.kv_heads = KVH;
