@@ -74,7 +74,7 @@ struct PCfg {
 // Barriers and small exchanges, behind the tiles.
 template <int ST, int RAW>
 struct PShared {
-  uint64_t full[ST], empty[ST], qfull, qempty, s[2][2], p[2][2], o[2], drain;
+  uint64_t full[ST], empty[ST], qfull, qempty, s[2][2], p[2][2], o[2], done[2], drain;
   uint64_t raw[4][RAW];              // a loader warp's e4m3 pages
   uint32_t tmem;
   volatile int bad;                  // a bad page was seen: the softmax checks pages from then on
@@ -239,6 +239,8 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
     }
     mbar_init(smem_u32(&sh.o[0]), 1);
     mbar_init(smem_u32(&sh.o[1]), 1);
+    mbar_init(smem_u32(&sh.done[0]), 1);
+    mbar_init(smem_u32(&sh.done[1]), 1);
     mbar_init(smem_u32(&sh.drain), 1);
     for (int i = 0; i < 4 * RAW; ++i) mbar_init(smem_u32(&sh.raw[0][0] + i), 1);
     fence_mbar_init();
@@ -284,6 +286,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
     const float c = fmaxf(rsqrtf(static_cast<float>(D)) * LOG2E * fabsf(sk), 1e-30f);
     uint32_t sph = 0;  // parities of the two S buffers
     uint32_t oph = 0;  // parity of the next P V
+    uint32_t dph = 0;  // parity of the next segment's end
     bool alive = true;
     for (int g = g0; g < g1 && alive;) {
       PrefixSeg sg;
@@ -340,8 +343,9 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
           const float al = (m == NEG_INF) ? 0.f : ex2(m - mn);
           l *= al;
           if (j > 0) {
-            // the previous item's P V (S of this item says that the one before
-            // it is complete)
+            // The previous item's P V.  S of this item was issued behind the one
+            // before that, and this item's waits for our P: o[s] is in the phase
+            // waited for or in the next.
             if (!(alive = wait(&sh.o[s], oph ^ 1u))) break;
             tc_fence_after();
             uint32_t o[16];
@@ -397,10 +401,10 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
       }
       if (!alive) break;
       const long long rec = static_cast<long long>(sg.seg) * 2 + s;
-      // The last P V.  S of the last item only says that the third last P V is
-      // complete, and a parity tells two neighbouring ones apart: one at a time.
-      if (ni > 1 && !(alive = wait(&sh.o[s], oph))) break;
-      if (!(alive = wait(&sh.o[s], oph ^ 1u))) break;
+      // The last P V, on a barrier of its own: o[s] may be one or two phases
+      // behind here, which a parity does not tell apart.
+      if (!(alive = wait(&sh.done[s], dph))) break;
+      dph ^= 1u;
       tc_fence_after();
       const bool valid = trow < p.rows;
       if (valid) p.ml[rec * PROWS + row] = make_float2(m == NEG_INF ? NEG_INF : m - BIAS, l);
@@ -671,13 +675,14 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
       }
     };
     // O (+)= P V of stream s, item buffer buf: 64 rows of V at v_addr
-    auto pv = [&](int s, int buf, uint32_t v_addr, bool first) {
+    auto pv = [&](int s, int buf, uint32_t v_addr, bool first, bool last) {
       const uint32_t v_lo = desc_lo(v_addr, HALF_BYTES);
       if (leader) {
 #pragma unroll
         for (int k = 0; k < PITEM / 16; ++k)
           mma_ts(256 + s * D, s * 128 + buf * PITEM + 8 * k, v_lo + k * (2048 >> 4), idPV, !first || k > 0);
         mma_commit(smem_u32(&sh.o[s]));
+        if (last) mma_commit(smem_u32(&sh.done[s]));
       }
     };
     for (int g = g0; g < g1 && alive;) {
@@ -725,7 +730,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
           if (!(alive = wait(&sh.p[s][buf], (pph[s] >> buf) & 1u))) break;
           pph[s] ^= 1u << buf;
           tc_fence_after();
-          pv(s, buf, v_addr + half_of(s, j), j == 0);
+          pv(s, buf, v_addr + half_of(s, j), j == 0, j + 1 == ni);
           if (s == 1 && last_use) give_back(stage);
           if (more) {
             if (s == 0 && first_use && !(alive = wait(&sh.full[ks], kph))) break;
