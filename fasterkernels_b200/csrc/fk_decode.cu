@@ -598,14 +598,20 @@ int own_part_prepare(OwnPart* own, const fk_prefix_args& a, void* workspace, int
   return FK_OK;
 }
 
-int own_part_zero_words(const OwnPart&, size_t ws_bytes) {
-  return static_cast<int>(64 + (ws_bytes > 256 ? (ws_bytes - 256) / SEG_BYTES : 0));  // header + counters (WsLayout)
-}
-
-int own_part_launch(OwnPart& own, float2* ml, float* acc, size_t ws_bytes, cudaStream_t stream) {
-  own.p.part_ml = ml;
-  own.p.part_acc = acc;
-  return launch<PAGED>(own.p, own.kv, own.device, ws_bytes, stream);
+int own_part_launch(OwnPart& own, int2* info, size_t ws_bytes, cudaStream_t stream, OwnRecords* r) {
+  Params& p = own.p;
+  p.part_info = info;
+  const int rc = launch<PAGED>(p, own.kv, own.device, ws_bytes, stream);
+  if (rc != FK_OK) return rc;
+  const int hp = hp_for(p.kv_heads, p.qc, own.kv, p.q_al16, p.G);
+  r->ml = reinterpret_cast<const float2*>(p.ws + p.ws_ml);
+  r->acc = reinterpret_cast<const float*>(p.ws + p.ws_acc);
+  r->info = info;
+  r->hp = hp;
+  r->qc = p.qc;
+  r->slots = hp == 4 ? 4 * GPAD : GMAX;
+  r->per_seq = p.qc == 1 ? p.kv_heads / hp : hp == 2 ? p.kv_heads * ((p.qc + 1) / 2) : p.kv_heads * p.qc;
+  return FK_OK;
 }
 
 void debug_settings(unsigned long long* wait_ns, int* inject) {

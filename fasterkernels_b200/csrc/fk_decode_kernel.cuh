@@ -199,11 +199,10 @@ struct Params {
   int o_al8;   // out base and strides 8-byte aligned (four outputs per store)
   int qc;      // query chunks of at most 8 heads per KV head: ceil(G / 8)
   int head_dim;  // D (the kernel is instantiated per D; kept for host checks)
-  // Own part of a shared-prefix decode: when set, the running (max, sum) and
-  // accumulators of each (sequence, query head) are stored here instead of
-  // being normalised into `out`.
-  float2* part_ml;
-  float* part_acc;
+  // Own part of a shared-prefix decode: when set, every segment, of whole items
+  // too, stays in the workspace for the join, item i's being records i + x .. i +
+  // x + y - 1 of part_info[i] = (x, y); nothing is merged or written to `out`.
+  int2* part_info;
   unsigned long long wait_ns;  // bound of every mbarrier wait
   int inject;                  // test hook: 1 = each CTA's producer withholds its first stage
 };
@@ -847,9 +846,8 @@ __global__ void __launch_bounds__(THREADS, KvCfg<KV, D, CP>::MINB) decode_split_
     for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
       long long t0;
       if (seq_len<LAYOUT>(p, b, &t0) == 0) {
-        if (LAYOUT == PAGED && p.part_ml != nullptr) {
-          for (int qh = et; qh < p.q_heads; qh += ETHREADS)
-            p.part_ml[static_cast<long long>(b) * p.q_heads + qh] = make_float2(NEG_INF, 0.f);
+        if (LAYOUT == PAGED && p.part_info != nullptr) {
+          for (int i = et; i < KVI; i += ETHREADS) p.part_info[static_cast<long long>(b) * KVI + i] = make_int2(0, 0);
           continue;
         }
         for (int qh = 0; qh < p.q_heads; ++qh)
@@ -890,7 +888,8 @@ __global__ void __launch_bounds__(THREADS, KvCfg<KV, D, CP>::MINB) decode_split_
         break;
       }
       const EpiSlot& E = eslot[eb];
-      const bool whole = (mt.flags & F_WHOLE) != 0;
+      const bool part = LAYOUT == PAGED && p.part_info != nullptr;
+      const bool whole = (mt.flags & F_WHOLE) != 0 && !part;
       const long long item = static_cast<long long>(mt.b) * KVI + mt.h;
       const long long obase = static_cast<long long>(mt.b) * p.o_sb;
       // One unit per thread and round: query head hd of KV head hh (head
@@ -926,13 +925,7 @@ __global__ void __launch_bounds__(THREADS, KvCfg<KV, D, CP>::MINB) decode_split_
         }
         const int qh = item_q<HP>(p, mt.h, hh, hd);
         const int hs = hh * GPAD + hd;  // head slot in a segment record
-        if (LAYOUT == PAGED && whole && p.part_ml != nullptr) {
-          const long long pr = static_cast<long long>(mt.b) * p.q_heads + qh;
-          float4* dst = reinterpret_cast<float4*>(p.part_acc + pr * D + d4);
-#pragma unroll
-          for (int k = 0; k < D / 32; ++k) dst[8 * k] = A[k];
-          if ((u & 7) == 0) p.part_ml[pr] = make_float2(M, L);
-        } else if (whole) {
+        if (whole) {
           float e, Lf;
           sink_norm(L, M, p.s_aux, qh, &e, &Lf);
           const long long ob = obase + static_cast<long long>(qh) * p.o_sh + d4;
@@ -956,6 +949,10 @@ __global__ void __launch_bounds__(THREADS, KvCfg<KV, D, CP>::MINB) decode_split_
       if (++eb == C::NSLOT) {
         eb = 0;
         eph ^= 1u;
+      }
+      if (part) {
+        if (et == 0) p.part_info[item] = make_int2(mt.c0, mt.nseg);
+        continue;
       }
       if (whole) continue;
       __threadfence();
@@ -1016,14 +1013,6 @@ __global__ void __launch_bounds__(THREADS, KvCfg<KV, D, CP>::MINB) decode_split_
           M = Mn;
         }
         const int qh = item_q<HP>(p, mt.h, hh, hd);
-        if (LAYOUT == PAGED && p.part_ml != nullptr) {
-          const long long pr = static_cast<long long>(mt.b) * p.q_heads + qh;
-          float4* dst = reinterpret_cast<float4*>(p.part_acc + pr * D + d0);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) dst[i] = make_float4(A[4 * i], A[4 * i + 1], A[4 * i + 2], A[4 * i + 3]);
-          if (d0 == 0) p.part_ml[pr] = make_float2(M, L);
-          continue;
-        }
         const long long ob = obase + static_cast<long long>(qh) * p.o_sh + d0;
         float e, Lf;
         sink_norm(L, M, p.s_aux, qh, &e, &Lf);

@@ -3,8 +3,8 @@
 // Sequence b attends the prefix's P tokens and then its own.  Softmax
 // statistics join by log-sum-exp, so the two parts are computed apart: the
 // prefix once for the whole batch (below), the own tokens by the split-KV
-// decode kernel (fk_decode_kernel.cuh), which stores its running (max, sum,
-// acc) instead of an output; a last kernel joins them with the sink.
+// decode kernel (fk_decode_kernel.cuh), which leaves its segments' (max, sum,
+// acc) in the workspace; a last kernel joins them all with the sink.
 //
 // Prefix part.  For one KV head the batch's query heads are the rows of a
 // matrix: row r = b * G + g, R = B * G rows, and the work is S = Q K^T (R x P),
@@ -42,6 +42,8 @@
 // anything, and 0 x NaN would reach the output).
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "fk_decode_kernel.cuh"
 #include "fk_host.h"
 #include "fk_prefix.h"
@@ -50,7 +52,7 @@
 namespace fk {
 
 #ifndef PSHARE
-#define PSHARE 3
+#define PSHARE 1
 #endif
 constexpr int SOFT_WARPS = 8;  // warps 0-7: softmax; 8-11 loaders; 12 MMA issue
 constexpr int LOAD_WARP = SOFT_WARPS, MMA_WARP = SOFT_WARPS + 4;
@@ -66,8 +68,8 @@ struct PCfg {
   static constexpr bool FP8 = KV == FK_DTYPE_E4M3;
   static constexpr int NH = D / 64;
   static constexpr int TILE_BYTES = NH * HALF_BYTES;  // Q, K or V tile in 16 bits
-  static constexpr int STAGES = D == 64 ? 8 : FP8 ? 3 : 5;
-  static constexpr int RAW = FP8 ? 4 : 0;             // e4m3 tiles on the way
+  static constexpr int STAGES = D == 64 ? 8 : FP8 ? 4 : 5;
+  static constexpr int RAW = FP8 ? 2 : 0;             // e4m3 tiles on the way
   static constexpr int TILES = (2 + STAGES) * TILE_BYTES + RAW * HALF_BYTES;
 };
 
@@ -102,8 +104,7 @@ struct PrefixParams {
   const float* scale_k;
   float2* ml;
   float* acc;
-  int* zero;            // the own part's status word and arrival counters
-  int zero_words;
+  int* own_status;      // the own part's status word, cleared here
   int* status;          // or null
   unsigned long long wait_ns;
   int inject;
@@ -257,7 +258,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
   const uint32_t tmem = 0;  // all 512 columns are ours, so the allocation starts at column 0
   grid_dependency_wait();
   grid_dependency_trigger();
-  for (int i = blockIdx.x * PTHREADS + tid; i < p.zero_words; i += gridDim.x * PTHREADS) p.zero[i] = 0;
+  if (blockIdx.x == 0 && tid == 0) *p.own_status = 0;
 
   bool past;
   const int plen = prefix_len(p.plen_dev, p.plen, p.blocks, &past);
@@ -285,8 +286,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
     // never 0: a masked logit (-inf) stays one
     const float c = fmaxf(rsqrtf(static_cast<float>(D)) * LOG2E * fabsf(sk), 1e-30f);
     uint32_t sph = 0;  // parities of the two S buffers
-    uint32_t oph = 0;  // parity of the next P V
-    uint32_t dph = 0;  // parity of the next segment's end
+    uint32_t oph = 0, dph = 0;  // parities of o (segments of more than one item) and done
     bool alive = true;
     for (int g = g0; g < g1 && alive;) {
       PrefixSeg sg;
@@ -343,10 +343,10 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
           const float al = (m == NEG_INF) ? 0.f : ex2(m - mn);
           l *= al;
           if (j > 0) {
-            // The previous item's P V.  S of this item was issued behind the one
-            // before that, and this item's waits for our P: o[s] is in the phase
-            // waited for or in the next.
-            if (!(alive = wait(&sh.o[s], oph ^ 1u))) break;
+            // The previous item's P V is complete once S of the next item is,
+            // which was issued behind it (no more than looked at here); the last
+            // item has no next one, o[s] stands in for it.
+            if (!(alive = j + 1 < ni ? wait(&sh.s[s][buf ^ 1], (sph >> (buf ^ 1)) & 1u) : wait(&sh.o[s], oph))) break;
             tc_fence_after();
             uint32_t o[16];
 #pragma unroll 1
@@ -397,12 +397,11 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh.p[s][buf]));
-        oph ^= 1u;
       }
       if (!alive) break;
+      if (ni > 1) oph ^= 1u;
       const long long rec = static_cast<long long>(sg.seg) * 2 + s;
-      // The last P V, on a barrier of its own: o[s] may be one or two phases
-      // behind here, which a parity does not tell apart.
+      // the last P V
       if (!(alive = wait(&sh.done[s], dph))) break;
       dph ^= 1u;
       tc_fence_after();
@@ -629,8 +628,12 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
               e4m3x4_to_f16x2x2(x[k].y, w[2], w[3]);
               e4m3x4_to_f16x2x2(x[k].z, w[4], w[5]);
               e4m3x4_to_f16x2x2(x[k].w, w[6], w[7]);
-              sts128(dst + r * 128 + ((c0 ^ (r & 7)) << 4), w[0], w[1], w[2], w[3]);
-              sts128(dst + r * 128 + (((c0 + 1) ^ (r & 7)) << 4), w[4], w[5], w[6], w[7]);
+              // lanes of the upper half store their second chunk first: a row's
+              // eight lanes then fill eight different 16-byte columns at a time
+              const uint32_t d0 = dst + r * 128 + ((c0 ^ (r & 7)) << 4), d1 = dst + r * 128 + (((c0 + 1) ^ (r & 7)) << 4);
+              const bool up = ch >= 4;
+              sts128(up ? d1 : d0, up ? w[4] : w[0], up ? w[5] : w[1], up ? w[6] : w[2], up ? w[7] : w[3]);
+              sts128(up ? d0 : d1, up ? w[0] : w[4], up ? w[1] : w[5], up ? w[2] : w[6], up ? w[3] : w[7]);
             }
             // also orders the reads of the raw slot before its next copy
             fence_async_proxy();
@@ -675,14 +678,14 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
       }
     };
     // O (+)= P V of stream s, item buffer buf: 64 rows of V at v_addr
-    auto pv = [&](int s, int buf, uint32_t v_addr, bool first, bool last) {
+    auto pv = [&](int s, int buf, uint32_t v_addr, int j, int ni) {
       const uint32_t v_lo = desc_lo(v_addr, HALF_BYTES);
       if (leader) {
 #pragma unroll
         for (int k = 0; k < PITEM / 16; ++k)
-          mma_ts(256 + s * D, s * 128 + buf * PITEM + 8 * k, v_lo + k * (2048 >> 4), idPV, !first || k > 0);
-        mma_commit(smem_u32(&sh.o[s]));
-        if (last) mma_commit(smem_u32(&sh.done[s]));
+          mma_ts(256 + s * D, s * 128 + buf * PITEM + 8 * k, v_lo + k * (2048 >> 4), idPV, j > 0 || k > 0);
+        if (j + 2 == ni) mma_commit(smem_u32(&sh.o[s]));
+        if (j + 1 == ni) mma_commit(smem_u32(&sh.done[s]));
       }
     };
     for (int g = g0; g < g1 && alive;) {
@@ -730,7 +733,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
           if (!(alive = wait(&sh.p[s][buf], (pph[s] >> buf) & 1u))) break;
           pph[s] ^= 1u << buf;
           tc_fence_after();
-          pv(s, buf, v_addr + half_of(s, j), j == 0, j + 1 == ni);
+          pv(s, buf, v_addr + half_of(s, j), j, ni);
           if (s == 1 && last_use) give_back(stage);
           if (more) {
             if (s == 0 && first_use && !(alive = wait(&sh.full[ks], kph))) break;
@@ -768,8 +771,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
 struct JoinParams {
   const float2* ml;       // prefix segments
   const float* acc;
-  const float2* own_ml;   // [B, QH]
-  const float* own_acc;   // [B, QH, D]
+  OwnRecords own;
   const int* plen_dev;
   int plen, blocks, rows, G, kv_heads, q_heads, ctas;
   const float* s_aux;
@@ -783,7 +785,8 @@ struct JoinParams {
 };
 
 constexpr int JTHREADS = 128;
-constexpr int JBATCH = 8;
+constexpr int JBATCH = 8;  // prefix records of a row in flight
+constexpr int JOWN = 4;    // own records
 
 template <int D>
 __global__ void __launch_bounds__(JTHREADS) join_kernel(const __grid_constant__ JoinParams p) {
@@ -798,9 +801,10 @@ __global__ void __launch_bounds__(JTHREADS) join_kernel(const __grid_constant__ 
   const int d0 = (blockIdx.y * (JTHREADS / p.rb) + threadIdx.x / p.rb) * 4;
   if (grow >= p.rows || d0 >= D) return;
   const int b = grow / p.G, qh = h * p.G + grow % p.G;
-  const long long orow = static_cast<long long>(b) * p.q_heads + qh;
-  const float2 own = __ldcg(p.own_ml + orow);
-  const float4 own_a = __ldcg(reinterpret_cast<const float4*>(p.own_acc + orow * D + d0));
+  int item, slot;
+  p.own.find(h, grow % p.G, &item, &slot);
+  const long long oitem = static_cast<long long>(b) * p.own.per_seq + item;
+  const int2 own = __ldcg(p.own.info + oitem);  // needed last: the prefix's records are read meanwhile
   bool past;
   const int plen = prefix_len(p.plen_dev, p.plen, p.blocks, &past);
   const PrefixPlan pl(plen, p.rows, p.kv_heads, p.ctas);
@@ -818,27 +822,12 @@ __global__ void __launch_bounds__(JTHREADS) join_kernel(const __grid_constant__ 
 
   float M = NEG_INF, L = 0.f;
   float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-  // a part with nothing in it (max -inf) may have unwritten accumulators
-  if (own.x != NEG_INF) {
-    M = own.x;
-    L = own.y;
-    A = own_a;
-  }
-  for (int i = 0; i < nrec; i += JBATCH) {
-    float2 ml[JBATCH];
-    float4 av[JBATCH];
-#pragma unroll
-    for (int k = 0; k < JBATCH; ++k) {
-      const bool ok = i + k < nrec;
-      const long long rec = rec0 + static_cast<long long>(ok ? i + k : i) * rstep;
-      ml[k] = __ldcg(p.ml + rec * PROWS + row);
-      av[k] = __ldcg(reinterpret_cast<const float4*>(p.acc + rec * PROWS * D) + (d0 / 4) * PROWS + row);
-      if (!ok) ml[k].x = NEG_INF;
-    }
+  auto merge = [&](const auto& ml, const auto& av, auto count) {
+    constexpr int N = decltype(count)::value;
     float Mn = M;
 #pragma unroll
-    for (int k = 0; k < JBATCH; ++k) Mn = fmaxf(Mn, ml[k].x);
-    if (Mn == NEG_INF) continue;
+    for (int k = 0; k < N; ++k) Mn = fmaxf(Mn, ml[k].x);
+    if (Mn == NEG_INF) return;
     const float sc = exp2f(M - Mn);
     L *= sc;
     A.x *= sc;
@@ -846,8 +835,8 @@ __global__ void __launch_bounds__(JTHREADS) join_kernel(const __grid_constant__ 
     A.z *= sc;
     A.w *= sc;
 #pragma unroll
-    for (int k = 0; k < JBATCH; ++k) {
-      if (ml[k].x == NEG_INF) continue;
+    for (int k = 0; k < N; ++k) {
+      if (ml[k].x == NEG_INF) continue;  // nothing attended: the accumulators may be unwritten
       const float e = exp2f(ml[k].x - Mn);
       L += e * ml[k].y;
       A.x += e * av[k].x;
@@ -856,6 +845,32 @@ __global__ void __launch_bounds__(JTHREADS) join_kernel(const __grid_constant__ 
       A.w += e * av[k].w;
     }
     M = Mn;
+  };
+  const float2 none = make_float2(NEG_INF, 0.f);
+  const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < nrec; i += JBATCH) {
+    float2 ml[JBATCH];
+    float4 av[JBATCH];
+#pragma unroll
+    for (int k = 0; k < JBATCH; ++k) {
+      const bool ok = i + k < nrec;
+      const long long rec = rec0 + static_cast<long long>(i + k) * rstep;
+      ml[k] = ok ? __ldcg(p.ml + rec * PROWS + row) : none;
+      av[k] = ok ? __ldcg(reinterpret_cast<const float4*>(p.acc + rec * PROWS * D) + (d0 / 4) * PROWS + row) : zero;
+    }
+    merge(ml, av, std::integral_constant<int, JBATCH>{});
+  }
+  for (int i = 0; i < own.y; i += JOWN) {
+    float2 ml[JOWN];
+    float4 av[JOWN];
+#pragma unroll
+    for (int k = 0; k < JOWN; ++k) {
+      const bool ok = i + k < own.y;
+      const long long rec = (oitem + own.x + i + k) * p.own.slots + slot;
+      ml[k] = ok ? __ldcg(p.own.ml + rec) : none;
+      av[k] = ok ? __ldcg(reinterpret_cast<const float4*>(p.own.acc + rec * HEAD_DIM + d0)) : zero;
+    }
+    merge(ml, av, std::integral_constant<int, JOWN>{});
   }
   float e, Lf;
   if (M == NEG_INF) e = 0.f, Lf = 0.f;  // nothing attended: zeros, whatever the sink
@@ -891,18 +906,17 @@ int prefix_ctas(int device) {
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
-// [own part's decode workspace | own (max, sum) | own acc | prefix (max, sum) | prefix acc]
+// [own part's decode workspace | its items' records | prefix (max, sum) | prefix acc]
 struct PrefixWs {
-  size_t own, own_ml, own_acc, ml, acc, total;
+  size_t own, info, ml, acc, total;
   PrefixWs(int device, int batch, int q_heads, int kv_heads, int head_dim, int kv_dtype) {
     own = fk_decode_workspace_bytes_gqa(device, batch, q_heads, kv_heads, kv_dtype);
     const long long rows = static_cast<long long>(batch) * (q_heads / kv_heads);
     const size_t rt = static_cast<size_t>((rows + PROWS - 1) / PROWS);
     const size_t segs = static_cast<size_t>(prefix_ctas(device)) + static_cast<size_t>(kv_heads) * ((rt + 1) / 2);
-    const size_t heads = static_cast<size_t>(batch) * q_heads;
-    own_ml = up256(own);
-    own_acc = up256(own_ml + heads * sizeof(float2));
-    ml = up256(own_acc + heads * head_dim * sizeof(float));
+    const size_t items = static_cast<size_t>(batch) * q_heads;  // at most
+    info = up256(own);
+    ml = up256(info + items * sizeof(int2));
     acc = up256(ml + segs * 2 * PROWS * sizeof(float2));
     total = own == 0 ? 0 : up256(acc + segs * 2 * PROWS * head_dim * sizeof(float));
   }
@@ -994,8 +1008,7 @@ extern "C" int fk_paged_shared_prefix_decode(const fk_prefix_args* a, void* work
   p.scale_k = kv == FK_DTYPE_E4M3 ? static_cast<const float*>(a->scale_k) : nullptr;
   p.ml = reinterpret_cast<float2*>(ws + w.ml);
   p.acc = reinterpret_cast<float*>(ws + w.acc);
-  p.zero = reinterpret_cast<int*>(ws);
-  p.zero_words = own_part_zero_words(own, w.own);
+  p.own_status = reinterpret_cast<int*>(ws);
   p.status = static_cast<int*>(a->status);
   debug_settings(&p.wait_ns, &p.inject);
   // 16-bit: (64 dims, 16 slots, D / 64 halves, heads, pages), a box is one
@@ -1023,13 +1036,11 @@ extern "C" int fk_paged_shared_prefix_decode(const fk_prefix_args* a, void* work
   else if (kv == FK_DTYPE_BF16) rc = D == 64 ? launch_prefix<FK_DTYPE_BF16, 64>(p, ctas, device, st) : launch_prefix<FK_DTYPE_BF16, 128>(p, ctas, device, st);
   else rc = launch_prefix<FK_DTYPE_E4M3, 128>(p, ctas, device, st);
   if (rc != FK_OK) return rc;
-  rc = own_part_launch(own, reinterpret_cast<float2*>(ws + w.own_ml), reinterpret_cast<float*>(ws + w.own_acc), w.own, st);
-  if (rc != FK_OK) return rc;
   JoinParams j = {};
+  rc = own_part_launch(own, reinterpret_cast<int2*>(ws + w.info), w.own, st, &j.own);
+  if (rc != FK_OK) return rc;
   j.ml = p.ml;
   j.acc = p.acc;
-  j.own_ml = reinterpret_cast<const float2*>(ws + w.own_ml);
-  j.own_acc = reinterpret_cast<const float*>(ws + w.own_acc);
   j.plen_dev = p.plen_dev;
   j.plen = p.plen;
   j.blocks = p.blocks;

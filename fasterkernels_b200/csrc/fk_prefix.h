@@ -1,6 +1,6 @@
 // fk_prefix.h -- what fk_prefix.cu needs of fk_decode.cu: the own-tokens part
-// of a shared-prefix decode, run by the paged decode kernel with its running
-// (max, sum, acc) stored instead of an output.
+// of a shared-prefix decode, run by the paged decode kernel with its segments'
+// (max, sum, acc) left in the workspace for the join.
 #pragma once
 #include <mutex>
 
@@ -15,9 +15,27 @@ struct OwnPart {
 
 // Argument checks and tensor maps (FK_OK, or an error).
 int own_part_prepare(OwnPart* own, const fk_prefix_args& a, void* workspace, int* device);
-// Leading 32-bit words of its workspace that must be zero before the launch.
-int own_part_zero_words(const OwnPart& own, size_t ws_bytes);
-int own_part_launch(OwnPart& own, float2* ml, float* acc, size_t ws_bytes, cudaStream_t stream);
+// The records it leaves: those of item i are i + info[i].x .. (info[i].y of
+// them), each `slots` query-head slots of HEAD_DIM floats.
+struct OwnRecords {
+  const float2* ml;
+  const float* acc;
+  const int2* info;
+  int hp, qc, slots, per_seq;  // KV heads of an item, query chunks of a KV head, slots, items of a sequence
+  // Item (within its sequence) and slot of query head g of KV head h's group.
+  __device__ void find(int h, int g, int* item, int* slot) const {
+    if (qc == 1) {
+      *item = h / hp;
+      *slot = (h % hp) * GPAD + g;
+    } else {
+      const int c = g >> 3;
+      *item = hp == 2 ? h * ((qc + 1) >> 1) + (c >> 1) : h * qc + c;
+      *slot = (hp == 2 ? (c & 1) * GPAD : 0) + (g & 7);
+    }
+  }
+};
+// Only the first word of its workspace (the status) must be zero before.
+int own_part_launch(OwnPart& own, int2* info, size_t ws_bytes, cudaStream_t stream, OwnRecords* records);
 // A tensor map with 128-byte swizzle (fk_decode.cu).
 int encode_map(CUtensorMap* map, int kv, int rank, const void* base, const uint64_t* dims, const uint64_t* strides_b,
                const uint32_t* box);
