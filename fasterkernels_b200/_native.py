@@ -132,6 +132,12 @@ def stream_of(device: torch.device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def raw_stream(index: int) -> int:
+    """The current stream of device ``index`` as an address, without making a
+    ``torch.cuda.Stream`` (4 us of a call of 30)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 # ---------------------------------------------------------------- workspace
 _ws = {}
 _ws_retired = []

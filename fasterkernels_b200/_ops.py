@@ -100,8 +100,9 @@ def _addr(t):
 
 
 def _rows16(t):
-    """t, or a copy whose rows start on 16-byte boundaries (an unaligned or
-    inner-strided view)."""
+    """t, or a copy whose rows start on 16-byte boundaries."""
+    if t is None:
+        return None
     e = t.element_size()
     if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s * e % 16 == 0 for s in t.stride()[:-1]):
         return t
@@ -117,34 +118,50 @@ def rope_launch(q: torch.Tensor, k: torch.Tensor, v: Optional[torch.Tensor], cos
     T, QH, D = q.shape
     if T == 0:
         return
-    q, k = _rows16(q), _rows16(k)
-    R = max_pos = cos_row = sin_row = table = 0
+    q_t, q_h, q_d = q.stride()
+    k_t, k_h, k_d = k.stride()
+    qo_t, qo_h, _ = q_out.stride()
+    ko_t = ko_h = R = max_pos = cos_row = sin_row = table = 0
+    inner = q_d == 1 == k_d
+    if k_out is not None:
+        ko_t, ko_h, _ = k_out.stride()
     if cos is not None:
-        cos, sin = _rows16(cos), _rows16(sin)
-        R, max_pos, table = 2 * cos.shape[1], cos.shape[0], _WIDE_CODES[cos.dtype]
-        cos_row, sin_row = cos.stride(0), sin.stride(0)
-    if q_weight is not None:
-        q_weight = _rows16(q_weight)
-    if k_weight is not None:
-        k_weight = _rows16(k_weight)
-    qs, ks, qos = q.stride(), k.stride(), q_out.stride()
-    kos = (0, 0) if k_out is None else k_out.stride()
-    vs, kps, vps, pool_code, bt_b, bt_rows, blocks, pages = (0, 0), (0, 0, 0), (0, 0, 0), 0, 0, 0, 0, 0
+        (max_pos, R), table = cos.shape, _WIDE_CODES[cos.dtype]
+        cos_row, c_d = cos.stride()
+        sin_row, s_d = sin.stride()
+        inner = inner and c_d == 1 == s_d
+    v_t = v_h = kp_p = kp_h = kp_s = vp_p = vp_h = vp_s = pool_code = bt_b = bt_rows = blocks = pages = 0
     if k_pool is not None:
-        v = _rows16(v)
-        vs, kps, vps = v.stride(), k_pool.stride(), v_pool.stride()
+        v_t, v_h, v_d = v.stride()
+        inner = inner and v_d == 1
+        kp_p, kp_h, kp_s, _ = k_pool.stride()
+        vp_p, vp_h, vp_s, _ = v_pool.stride()
         pool_code, pages = N.dtype_code(k_pool.dtype), k_pool.shape[0]
-        bt_b, bt_rows, blocks = bt.stride(0), bt.shape[0], bt.shape[1]
-    args = _ROPE_ARGS.pack(
-        q.data_ptr(), k.data_ptr(), _addr(v), q_out.data_ptr(), _addr(k_out), _addr(k_pool), _addr(v_pool), _addr(cos),
-        _addr(sin), _addr(positions), _addr(seq_ids), _addr(bt), _addr(q_weight), _addr(k_weight), _addr(scale_k),
-        _addr(scale_v), _addr(status),
-        qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], qos[0], qos[1], kos[0], kos[1],
-        kps[0], kps[1], kps[2], vps[0], vps[1], vps[2], cos_row, sin_row, bt_b,
-        T, QH, k.shape[1], D, R, interleaved, max_pos, bt_rows, blocks, pages, N.dtype_code(q.dtype), pool_code, table,
-        0 if q_weight is None else _WIDE_CODES[q_weight.dtype], 0 if k_weight is None else _WIDE_CODES[k_weight.dtype],
-        eps)
-    N.check(N.lib().fk_qk_norm_rope(args, N.stream_of(q.device)), "fk_qk_norm_rope")
+        bt_rows, blocks = bt.shape
+        bt_b = bt.stride(0)
+    qw = kw = 0
+    if q_weight is not None:
+        qw = _WIDE_CODES[q_weight.dtype]
+    if k_weight is not None:
+        kw = _WIDE_CODES[k_weight.dtype]
+    if inner:
+        args = _ROPE_ARGS.pack(
+            q.data_ptr(), k.data_ptr(), _addr(v), q_out.data_ptr(), _addr(k_out), _addr(k_pool), _addr(v_pool), _addr(cos),
+            _addr(sin), _addr(positions), _addr(seq_ids), _addr(bt), _addr(q_weight), _addr(k_weight), _addr(scale_k),
+            _addr(scale_v), _addr(status), q_t, q_h, k_t, k_h, v_t, v_h, qo_t, qo_h, ko_t, ko_h, kp_p, kp_h, kp_s, vp_p, vp_h,
+            vp_s, cos_row, sin_row, bt_b, T, QH, k.shape[1], D, 2 * R, interleaved, max_pos, bt_rows, blocks, pages,
+            N.dtype_code(q.dtype), pool_code, table, qw, kw, eps)
+        rc = N.lib().fk_qk_norm_rope(args, N.raw_stream(q.device.index))
+        if rc == 0:
+            return
+    # rows the kernel cannot read in 16-byte pieces: copies of those inputs
+    ins = (q, k, v, cos, sin, q_weight, k_weight)
+    fit = tuple(_rows16(t) for t in ins)
+    if all(a is b for a, b in zip(ins, fit)):
+        N.check(rc, "fk_qk_norm_rope")
+    q, k, v, cos, sin, q_weight, k_weight = fit
+    rope_launch(q, k, v, cos, sin, positions, seq_ids, bt, q_weight, k_weight, eps, interleaved, scale_k, scale_v, q_out,
+                k_out, k_pool, v_pool, status)
 
 
 _PREFIX_ARGS = struct.Struct("13Q22q")  # fk_prefix_args of include/fk_decode.h
@@ -180,7 +197,8 @@ def shared_prefix_launch(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
         lens.data_ptr(), _addr(s_aux), out.data_ptr(), _addr(scale_q), _addr(scale_k), _addr(scale_v), status.data_ptr(),
         prefix_len_host, prefix_table.shape[0], B, QH, KVH, D, P, bt.shape[1], N.dtype_code(q.dtype), kv_code,
         N.dtype_code(out.dtype), qs[0], qs[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], bt.stride(0), os[0], os[1])
-    N.check(lib.fk_paged_shared_prefix_decode(args, N.ptr(ws), need, N.stream_of(dev)), "fk_paged_shared_prefix_decode")
+    N.check(lib.fk_paged_shared_prefix_decode(args, ws.data_ptr(), need, N.raw_stream(dev.index)),
+            "fk_paged_shared_prefix_decode")
 
 
 # ---------------------------------------------------------------- custom ops

@@ -15,7 +15,7 @@ from .. import _native as N
 from .. import _ops
 from ..gqa_decode import _check_idx
 from ..gqa_decode_hf import _scale_ptr
-from ..qk_norm_rope import _check_heads, _check_out, _check_status, _check_table, _check_weight
+from ..qk_norm_rope import _check_heads, _check_no_grad, _check_out, _check_status, _check_table, _check_weight
 
 
 def paged_kv_append_rope(q, k, v, k_pool, v_pool, block_table, positions, cos, sin, *, seq_ids=None, q_weight=None,
@@ -36,22 +36,20 @@ def paged_kv_append_rope(q, k, v, k_pool, v_pool, block_table, positions, cos, s
     ``status``, if given.  Returns the rotated q [T, Q_H, D]."""
     if q.dim() == 4 and k.dim() == 4 and v.dim() == 4 and q.shape[2] == k.shape[2] == v.shape[2] == 1:
         q, k, v = q.squeeze(2), k.squeeze(2), v.squeeze(2)
-    _check_heads(q, k, "paged_kv_append_rope")
-    dev = q.device
-    if v.shape != k.shape or v.dtype != k.dtype or v.device != dev:
+    T, D, dev = _check_heads(q, k, "paged_kv_append_rope")
+    shape, dt = k.shape, k.dtype
+    if v.shape != shape or v.dtype != dt or v.device != dev:
         raise ValueError("v must match k in shape, dtype and device")
-    if torch.is_grad_enabled() and v.requires_grad:
-        raise ValueError("paged_kv_append_rope has no backward pass; call it under torch.no_grad()")
-    T, _, D = q.shape
-    if (k_pool.dim() != 4 or k_pool.shape != v_pool.shape or k_pool.shape[1] != k.shape[1] or k_pool.shape[2] != 16
-            or k_pool.shape[3] != D):
+    _check_no_grad("paged_kv_append_rope", q, k, v, q_weight, k_weight)
+    pool, pdt = k_pool.shape, k_pool.dtype
+    if len(pool) != 4 or pool != v_pool.shape or pool[1] != shape[1] or pool[2] != 16 or pool[3] != D:
         raise ValueError("pools must be [num_pages, KV_H, 16, D] with the heads and head dim of k")
-    if k_pool.dtype != v_pool.dtype or k_pool.device != dev or v_pool.device != dev:
+    if v_pool.dtype != pdt or k_pool.device != dev or v_pool.device != dev:
         raise ValueError("the pools must have one dtype and be on q's device")
     if k_pool.stride(-1) != 1 or v_pool.stride(-1) != 1:
         raise ValueError("the pools must have unit inner stride")
-    pool_code = N.dtype_code(k_pool.dtype)
-    if pool_code != N.FK_DTYPE_E4M3 and k_pool.dtype != k.dtype:
+    pool_code = N.dtype_code(pdt)
+    if pool_code != N.FK_DTYPE_E4M3 and pdt != dt:
         raise TypeError("a 16-bit pool must have the dtype of k and v")
     if block_table.dim() != 2 or block_table.device != dev:
         raise ValueError("block_table must be [B, max_blocks] on q's device")
@@ -68,8 +66,8 @@ def paged_kv_append_rope(q, k, v, k_pool, v_pool, block_table, positions, cos, s
     if positions.numel() != T:
         raise ValueError("positions must have one entry per token")
     _check_table(cos, sin, D, dev)
-    qw = _check_weight(q_weight, "q_weight", D, dev)
-    kw = _check_weight(k_weight, "k_weight", D, dev)
+    _check_weight(q_weight, "q_weight", D, dev)
+    _check_weight(k_weight, "k_weight", D, dev)
     sk = sv = None
     if pool_code == N.FK_DTYPE_E4M3:
         if scale_k is None or scale_v is None:
@@ -79,6 +77,6 @@ def paged_kv_append_rope(q, k, v, k_pool, v_pool, block_table, positions, cos, s
     if k_out is not None:
         k_out = _check_out(k_out, k, "k_out")
     _check_status(status, dev)
-    _ops.rope(q, k, v, cos, sin, positions, seq_ids, bt, qw, kw, float(eps), bool(interleaved), sk, sv, q_out, k_out,
+    _ops.rope(q, k, v, cos, sin, positions, seq_ids, bt, q_weight, k_weight, float(eps), bool(interleaved), sk, sv, q_out, k_out,
               k_pool, v_pool, status)
     return q_out

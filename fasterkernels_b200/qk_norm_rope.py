@@ -35,56 +35,61 @@ def rope_table(max_positions: int, rotary_dim: int, base: float = 10000.0, *, in
 
 
 def _check_heads(q, k, name):
+    """(tokens, head dim, device) of q and k, checked."""
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError("q and k must be [T, Q_H, D] and [T, KV_H, D]")
     if not q.is_cuda:
         raise ValueError(f"{name} runs on CUDA tensors only")
-    if k.device != q.device:
+    dev, dt = q.device, q.dtype
+    if k.device != dev:
         raise ValueError("q and k must be on the same device")
-    if q.dtype not in _HALF or k.dtype != q.dtype:
+    if dt not in _HALF or k.dtype != dt:
         raise TypeError("q and k must both be float16 or bfloat16")
     T, QH, D = q.shape
-    if k.shape[0] != T or k.shape[2] != D:
+    Tk, KH, Dk = k.shape
+    if Tk != T or Dk != D:
         raise ValueError("q and k must have the same tokens and head dim")
     if D not in HEAD_DIMS:
         raise ValueError(f"head_dim must be one of {HEAD_DIMS}")
-    if QH == 0 or k.shape[1] == 0:
+    if QH == 0 or KH == 0:
         raise ValueError("q and k must have heads")
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
-        raise ValueError(f"{name} has no backward pass; call it under torch.no_grad()")
+    return T, D, dev
+
+
+def _check_no_grad(name, *tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{name} has no backward pass; call it under torch.no_grad()")
 
 
 def _check_table(cos, sin, D, dev):
-    """Rows of the tables and the rotated dims (0: no rotation)."""
-    if cos is None and sin is None:
-        return 0
+    """The rotated dims (0: no rotation)."""
     if cos is None or sin is None:
-        raise ValueError("cos and sin go together")
-    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != sin.dtype or cos.dtype not in _TABLE:
+        if cos is not None or sin is not None:
+            raise ValueError("cos and sin go together")
+        return 0
+    dt, shape = cos.dtype, cos.shape
+    if len(shape) != 2 or sin.shape != shape or sin.dtype != dt or dt not in _TABLE:
         raise ValueError("cos and sin must be [max_positions, rotary_dim / 2] of one type: float32, float16 or bfloat16")
     if cos.device != dev or sin.device != dev:
         raise ValueError("cos and sin must be on q's device")
-    R = 2 * cos.shape[1]
+    R = 2 * shape[1]
     if R == 0 or R > D or R % 16:
         raise ValueError("rotary_dim (2 * cos.shape[1]) must be a multiple of 16 up to the head dim")
-    if cos.shape[0] == 0:
+    if shape[0] == 0:
         raise ValueError("the cos / sin tables must have rows")
     return R
 
 
 def _check_weight(w, name, D, dev):
-    if w is None:
-        return None
-    if w.device != dev or w.numel() != D or w.dtype not in _TABLE:
+    if w is not None and (w.device != dev or w.numel() != D or w.dtype not in _TABLE):
         raise ValueError(f"{name} must have head_dim entries (float32, float16 or bfloat16) on q's device")
-    if torch.is_grad_enabled() and w.requires_grad:
-        raise ValueError(f"{name} requires grad; the operator has no backward pass, call it under torch.no_grad()")
-    return w.detach()
 
 
 def _check_out(out, like, name):
     if out is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+        return like.new_empty(like.shape)
     if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device or out.stride(-1) != 1:
         raise ValueError(f"{name} must have the shape, dtype and device of its input, with unit inner stride")
     return out
@@ -111,9 +116,8 @@ def qk_norm_rope(q, k, cos, sin, positions=None, *, q_weight=None, k_weight=None
     A position outside the tables zeroes the token's rows and sets
     FK_STATUS_BAD_POSITION in ``status`` (an int32 device tensor), if given.
     Returns (q_out, k_out)."""
-    _check_heads(q, k, "qk_norm_rope")
-    dev = q.device
-    T, _, D = q.shape
+    T, D, dev = _check_heads(q, k, "qk_norm_rope")
+    _check_no_grad("qk_norm_rope", q, k, q_weight, k_weight)
     R = _check_table(cos, sin, D, dev)
     if positions is not None:
         positions = _check_idx(positions, "positions", dev)
@@ -121,13 +125,13 @@ def qk_norm_rope(q, k, cos, sin, positions=None, *, q_weight=None, k_weight=None
             raise ValueError("positions must have one entry per token")
     elif R == 0:
         positions = torch.zeros(T, dtype=torch.int32, device=dev)
-    qw = _check_weight(q_weight, "q_weight", D, dev)
-    kw = _check_weight(k_weight, "k_weight", D, dev)
+    _check_weight(q_weight, "q_weight", D, dev)
+    _check_weight(k_weight, "k_weight", D, dev)
     q_out = _check_out(q_out, q, "q_out")
     k_out = _check_out(k_out, k, "k_out")
     _check_status(status, dev)
-    _ops.rope(q, k, None, cos, sin, positions, None, None, qw, kw, float(eps), bool(interleaved), None, None, q_out, k_out,
-              None, None, status)
+    _ops.rope(q, k, None, cos, sin, positions, None, None, q_weight, k_weight, float(eps), bool(interleaved), None, None,
+              q_out, k_out, None, None, status)
     return q_out, k_out
 
 
