@@ -365,6 +365,7 @@ void fill_common(Params& p, const void* q, int64_t sq_b, int64_t sq_h, void* out
   p.scale_k = scale_k;
   p.scale_v = scale_v;
   p.ws = static_cast<unsigned char*>(ws);
+  p.status = static_cast<int*>(ws);
   p.qc = qc_for(q_heads, kv_heads);
   p.o_al8 = ((reinterpret_cast<uintptr_t>(out) & 7) == 0 && (so_b & 3) == 0 && (so_h & 3) == 0) ? 1 : 0;
   const int64_t qes = (q_dtype == FK_DTYPE_E4M3) ? 1 : 2;
@@ -598,9 +599,10 @@ int own_part_prepare(OwnPart* own, const fk_prefix_args& a, void* workspace, int
   return FK_OK;
 }
 
-int own_part_launch(OwnPart& own, int2* info, size_t ws_bytes, cudaStream_t stream, OwnRecords* r) {
+int own_part_launch(OwnPart& own, int2* info, int* status, size_t ws_bytes, cudaStream_t stream, OwnRecords* r) {
   Params& p = own.p;
   p.part_info = info;
+  if (status != nullptr) p.status = status;  // else the workspace's first word, which nobody reads
   const int rc = launch<PAGED>(p, own.kv, own.device, ws_bytes, stream);
   if (rc != FK_OK) return rc;
   const int hp = hp_for(p.kv_heads, p.qc, own.kv, p.q_al16, p.G);
@@ -765,6 +767,7 @@ extern "C" int fk_flash_decode_gqa_varlen_noalloc(const void* q, const void* k_v
   void* scratch = nullptr;
   if ((rc = noalloc_scratch(device, &scratch)) != FK_OK) return rc;
   p.ws = static_cast<unsigned char*>(scratch);
+  p.status = static_cast<int*>(scratch);
   // The arrival counters must start at zero: clear them on the caller's
   // stream (a memset, not an allocation).  The status word before them is
   // left alone: it collects FK_STATUS_* bits until fk_noalloc_read_status

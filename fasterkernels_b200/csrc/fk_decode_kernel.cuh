@@ -203,6 +203,7 @@ struct Params {
   // too, stays in the workspace for the join, item i's being records i + x .. i +
   // x + y - 1 of part_info[i] = (x, y); nothing is merged or written to `out`.
   int2* part_info;
+  int* status;         // FK_STATUS_* word: the workspace's first, or the caller's
   unsigned long long wait_ns;  // bound of every mbarrier wait
   int inject;                  // test hook: 1 = each CTA's producer withholds its first stage
 };
@@ -416,7 +417,7 @@ __global__ void __launch_bounds__(THREADS, KvCfg<KV, D, CP>::MINB) decode_split_
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  WsHeader* hdr = reinterpret_cast<WsHeader*>(p.ws);
+  WsHeader* hdr = reinterpret_cast<WsHeader*>(p.status);
   int* cnt = reinterpret_cast<int*>(p.ws + p.ws_cnt);
   float2* ws_ml = reinterpret_cast<float2*>(p.ws + p.ws_ml);
   float* ws_acc = reinterpret_cast<float*>(p.ws + p.ws_acc);

@@ -104,7 +104,6 @@ struct PrefixParams {
   const float* scale_k;
   float2* ml;
   float* acc;
-  int* own_status;      // the own part's status word, cleared here
   int* status;          // or null
   unsigned long long wait_ns;
   int inject;
@@ -256,9 +255,12 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = 0;  // all 512 columns are ours, so the allocation starts at column 0
-  grid_dependency_wait();
+  // The kernel before this one in the stream is the own part's, which this one
+  // does not depend on: its blocks start as SMs come free and only wait for it
+  // before they end (so that the join, which waits for this kernel, finds both
+  // parts).  What both read was complete before: the own part's blocks let this
+  // kernel start after their own wait for what precedes them.
   grid_dependency_trigger();
-  if (blockIdx.x == 0 && tid == 0) *p.own_status = 0;
 
   bool past;
   const int plen = prefix_len(p.plen_dev, p.plen, p.blocks, &past);
@@ -758,6 +760,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  grid_dependency_wait();
   if (warp == MMA_WARP) tmem_dealloc(*const_cast<volatile uint32_t*>(&sh.tmem), 512);
 }
 
@@ -779,8 +782,6 @@ struct JoinParams {
   void* out;
   long long o_b, o_h;
   int out_dtype, o_al8;
-  const int* own_status;
-  int* status;
   int rb;  // rows of a block (a power of two); JTHREADS / rb groups of four dims
 };
 
@@ -792,8 +793,6 @@ template <int D>
 __global__ void __launch_bounds__(JTHREADS) join_kernel(const __grid_constant__ JoinParams p) {
   grid_dependency_wait();
   grid_dependency_trigger();
-  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0 && p.status != nullptr && *p.own_status != 0)
-    atomicOr(p.status, *p.own_status);
   const int per_head = (p.rows + p.rb - 1) / p.rb;
   const int h = blockIdx.x / per_head, first = blockIdx.x % per_head * p.rb;  // the block's first row
   const int tile = first / PROWS, row = first % PROWS + (threadIdx.x & (p.rb - 1));
@@ -1008,7 +1007,6 @@ extern "C" int fk_paged_shared_prefix_decode(const fk_prefix_args* a, void* work
   p.scale_k = kv == FK_DTYPE_E4M3 ? static_cast<const float*>(a->scale_k) : nullptr;
   p.ml = reinterpret_cast<float2*>(ws + w.ml);
   p.acc = reinterpret_cast<float*>(ws + w.acc);
-  p.own_status = reinterpret_cast<int*>(ws);
   p.status = static_cast<int*>(a->status);
   debug_settings(&p.wait_ns, &p.inject);
   // 16-bit: (64 dims, 16 slots, D / 64 halves, heads, pages), a box is one
@@ -1032,12 +1030,12 @@ extern "C" int fk_paged_shared_prefix_decode(const fk_prefix_args* a, void* work
   }
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   DeviceScope scope(device);
+  JoinParams j = {};
+  rc = own_part_launch(own, reinterpret_cast<int2*>(ws + w.info), p.status, w.own, st, &j.own);
+  if (rc != FK_OK) return rc;
   if (kv == FK_DTYPE_F16) rc = D == 64 ? launch_prefix<FK_DTYPE_F16, 64>(p, ctas, device, st) : launch_prefix<FK_DTYPE_F16, 128>(p, ctas, device, st);
   else if (kv == FK_DTYPE_BF16) rc = D == 64 ? launch_prefix<FK_DTYPE_BF16, 64>(p, ctas, device, st) : launch_prefix<FK_DTYPE_BF16, 128>(p, ctas, device, st);
   else rc = launch_prefix<FK_DTYPE_E4M3, 128>(p, ctas, device, st);
-  if (rc != FK_OK) return rc;
-  JoinParams j = {};
-  rc = own_part_launch(own, reinterpret_cast<int2*>(ws + w.info), w.own, st, &j.own);
   if (rc != FK_OK) return rc;
   j.ml = p.ml;
   j.acc = p.acc;
@@ -1056,8 +1054,6 @@ extern "C" int fk_paged_shared_prefix_decode(const fk_prefix_args* a, void* work
   j.o_h = a->o_h;
   j.out_dtype = static_cast<int>(a->out_dtype);
   j.o_al8 = own.p.o_al8;
-  j.own_status = reinterpret_cast<const int*>(ws);
-  j.status = p.status;
   j.rb = 8;
   while (j.rb < PROWS && j.rb < p.rows) j.rb *= 2;
   const dim3 grid(static_cast<unsigned>(KVH * ((p.rows + j.rb - 1) / j.rb)), static_cast<unsigned>((D / 4 * j.rb + JTHREADS - 1) / JTHREADS));

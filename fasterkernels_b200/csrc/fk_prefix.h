@@ -34,8 +34,8 @@ struct OwnRecords {
     }
   }
 };
-// Only the first word of its workspace (the status) must be zero before.
-int own_part_launch(OwnPart& own, int2* info, size_t ws_bytes, cudaStream_t stream, OwnRecords* records);
+// Nothing in its workspace need be set before.
+int own_part_launch(OwnPart& own, int2* info, int* status, size_t ws_bytes, cudaStream_t stream, OwnRecords* records);
 // A tensor map with 128-byte swizzle (fk_decode.cu).
 int encode_map(CUtensorMap* map, int kv, int rank, const void* base, const uint64_t* dims, const uint64_t* strides_b,
                const uint32_t* box);
