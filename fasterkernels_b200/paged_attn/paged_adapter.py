@@ -15,7 +15,9 @@ keyword, which transformers 5.x no longer passes) of layer
      ``value_states``) of all sequences with one ``paged_kv_append`` kernel
      (the reference loops over sequences with a ``.item()`` per token, :38-40);
   3. runs ``paged_flash_decode`` over the layer's pools (e4m3 pools use the
-     cache's ``k_scale``/``v_scale``; sinks come from ``module.sinks``);
+     cache's ``k_scale``/``v_scale``; sinks come from ``module.sinks``), or
+     ``paged_flash_decode_shared_prefix`` when the bound sequences hold the
+     pages of a common prefix that is worth it (``PagedKVCache.fork_sequence``);
   4. at the last layer, commits the step (``end_step``).
 Every layer of one step therefore sees the same lengths; the reference's
 ``append_kv`` advances a sequence's length once per layer call
@@ -39,6 +41,7 @@ import torch
 from ..gqa_decode_hf import _check_scaling, _fallback, _module_sinks
 from .paged_decode import paged_flash_decode
 from .paged_kv_cache import PAGE_SIZE, PagedKVCache
+from .shared_prefix import paged_flash_decode_shared_prefix, shared_prefix_pays
 
 
 @dataclass
@@ -48,6 +51,8 @@ class _Binding:
     write_prefill: bool = True
     lens: Optional[torch.Tensor] = None  # lengths of the step in progress (device)
     bt: Optional[torch.Tensor] = None    # block-table rows of the step in progress (device)
+    shared: int = 0                      # leading pages of a common prefix in this step (0: each sequence alone)
+    own: Optional[torch.Tensor] = None   # lengths without them
 
 
 _BOUND = _Binding()
@@ -59,8 +64,8 @@ def set_paged_attention_cache(cache: Optional[PagedKVCache], seq_ids: List[int],
     _BOUND.cache = cache
     _BOUND.seq_ids = list(seq_ids)
     _BOUND.write_prefill = bool(write_prefill)
-    _BOUND.lens = None
-    _BOUND.bt = None
+    _BOUND.lens = _BOUND.bt = _BOUND.own = None
+    _BOUND.shared = 0
 
 
 def get_paged_attention_cache() -> Tuple[Optional[PagedKVCache], List[int]]:
@@ -78,17 +83,24 @@ def custom_paged_attention_forward(module, query_states, key_states, value_state
             raise ValueError(f"bound {len(_BOUND.seq_ids)} sequence ids for a batch of {bsz}")
         if layer == 0 or _BOUND.lens is None:
             _BOUND.bt, _, _BOUND.lens = cache.begin_step(_BOUND.seq_ids)
+            pages = cache.shared_prefix_pages(_BOUND.seq_ids)
+            _BOUND.shared = pages if shared_prefix_pays(bsz, pages * PAGE_SIZE) else 0
+            _BOUND.own = _BOUND.lens - PAGE_SIZE * _BOUND.shared if _BOUND.shared else None
         cache.append_kv_batch(layer, key_states[:, :, -1], value_states[:, :, -1])
         e4m3 = cache.dtype == torch.float8_e4m3fn
-        out = paged_flash_decode(query_states.squeeze(2), cache.k_pool[layer], cache.v_pool[layer],
-                                 _BOUND.bt, _BOUND.lens, PAGE_SIZE,
-                                 s_aux=_module_sinks(module, q_heads, query_states.device),
-                                 scale_k=cache.k_scale if e4m3 else None, scale_v=cache.v_scale if e4m3 else None,
-                                 out_dtype=query_states.dtype if e4m3 else None)
+        kw = dict(s_aux=_module_sinks(module, q_heads, query_states.device),
+                  scale_k=cache.k_scale if e4m3 else None, scale_v=cache.v_scale if e4m3 else None,
+                  out_dtype=query_states.dtype if e4m3 else None)
+        q, kp, vp, n = query_states.squeeze(2), cache.k_pool[layer], cache.v_pool[layer], _BOUND.shared
+        if n:
+            out = paged_flash_decode_shared_prefix(q, kp, vp, _BOUND.bt[0, :n], n * PAGE_SIZE, _BOUND.bt[:, n:], _BOUND.own,
+                                                   PAGE_SIZE, **kw)
+        else:
+            out = paged_flash_decode(q, kp, vp, _BOUND.bt, _BOUND.lens, PAGE_SIZE, **kw)
         if layer == cache.num_layers - 1:
             cache.end_step()
-            _BOUND.lens = None
-            _BOUND.bt = None
+            _BOUND.lens = _BOUND.bt = _BOUND.own = None
+            _BOUND.shared = 0
         return out.unsqueeze(2), None
     if cache is not None and _BOUND.write_prefill and q_len > 1 and len(_BOUND.seq_ids) == bsz:
         for b, sid in enumerate(_BOUND.seq_ids):

@@ -1,0 +1,297 @@
+"""Sequences that share pages: PagedKVCache's bookkeeping (CPU), and the step of
+a layer as a server runs it (GPU): norm, rotate and append into forked
+sequences, decode behind the shared prefix, through the cache and through the
+paged adapter."""
+import pytest
+import torch
+
+import fasterkernels_b200 as fk
+from fasterkernels_b200.paged_attn import PAGE_SIZE, PagedKVCache, paged_kv_append
+from fasterkernels_b200.paged_attn.shared_prefix import shared_prefix_pays
+from _operator_refs import attention_bound, norm_rope_ref, shared_prefix_ref
+
+gpu = pytest.mark.gpu
+E4M3 = torch.float8_e4m3fn
+
+
+def make(pages=12, seqs=4, blocks=6, device="cpu", dtype=torch.float16, layers=2, heads=2, head_dim=128):
+    return PagedKVCache(num_layers=layers, num_pages=pages, max_seqs=seqs, max_blocks_per_seq=blocks, num_kv_heads=heads,
+                        head_dim=head_dim, dtype=dtype, device=device)
+
+
+def prefill(c, sid, n, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    k = torch.randn(c.num_kv_heads, n, c.head_dim, generator=g).to(c.dtype)
+    for layer in range(c.num_layers):
+        c.write_prefill(sid, layer, k, k)
+    return k
+
+
+# ------------------------------------------------------------------ CPU
+def test_fork_shares_full_pages_and_frees_them_with_the_last_holder():
+    c = make()
+    a = c.allocate_sequence()
+    prefill(c, a, 40)
+    assert c.pages_used == 3
+    b = c.fork_sequence(a, 32)
+    d = c.fork_sequence(b, 16)
+    assert c.pages_used == 3 and (c.seq_len(b), c.seq_len(d)) == (32, 16)
+    assert c.block_table[b].tolist()[:3] == c.block_table[a].tolist()[:2] + [-1]
+    assert (c.shared_prefix_pages([a, b]), c.shared_prefix_pages([a, b, d]), c.shared_prefix_pages([d, a])) == (2, 1, 1)
+    # new tokens go to pages of their own
+    bt, pos, lens = c.begin_step([a, b, d])
+    assert pos.tolist() == [40, 32, 16] and lens.tolist() == [41, 33, 17]
+    c.end_step()
+    assert c.pages_used == 5 and len(set(c._pages[b]) & set(c._pages[a])) == 2
+    assert c.shared_prefix_pages([a, b]) == 2
+    free = c.pages_free
+    c.free_sequence(a)  # b and d still hold its first pages
+    assert c.pages_free == free + 1
+    assert c.shared_prefix_pages([b, d]) == 1
+    c.free_sequence(d)
+    assert c.pages_free == free + 2
+    c.free_sequence(b)
+    assert c.pages_free == c.num_pages and sorted(c._free_pages) == list(range(c.num_pages)) and not c._page_refs
+
+
+def test_fork_refusals():
+    c = make()
+    a = c.allocate_sequence()
+    prefill(c, a, 40)
+    for n in (0, -16, 17, 48):
+        with pytest.raises(ValueError, match="multiple"):
+            c.fork_sequence(a, n)
+    with pytest.raises(ValueError, match="active"):
+        c.fork_sequence(3, 16)
+    with pytest.raises(ValueError, match="active"):
+        c.fork_sequence(99, 16)
+    for _ in range(3):
+        c.fork_sequence(a, 16)
+    with pytest.raises(RuntimeError, match="occupied"):
+        c.fork_sequence(a, 16)
+    assert all(n == 4 for n in c._page_refs.values())  # a refused fork takes no reference
+    with pytest.raises(RuntimeError, match="shared"):
+        prefill(c, a, 40)
+    with pytest.raises(RuntimeError, match="shared"):
+        prefill(c, 1, 5)
+
+
+def test_shared_prefix_of_unrelated_single_and_repeated_sequences():
+    c = make()
+    a, b = c.allocate_sequence(), c.allocate_sequence()
+    assert c.shared_prefix_pages([]) == 0 and c.shared_prefix_pages([a]) == 0 and c.shared_prefix_pages([a, b]) == 0
+    prefill(c, a, 40)
+    prefill(c, b, 40)
+    assert c.shared_prefix_pages([a, b]) == 0 and c.shared_prefix_pages([a]) == 2 and c.shared_prefix_pages([a, a]) == 2
+    assert not shared_prefix_pays(1, 10 ** 6) and not shared_prefix_pays(2, 0) and shared_prefix_pays(64, 32768)
+
+
+def test_begin_chunk_places_ragged_tokens_and_commits_their_counts():
+    c = make()
+    a, b, d = (c.allocate_sequence() for _ in range(3))
+    prefill(c, a, 14)
+    bt, pos, seq = c.begin_chunk([a, b, d], [5, 0, 17])
+    assert pos.tolist() == [14, 15, 16, 17, 18] + list(range(17)) and seq.tolist() == [0] * 5 + [2] * 17
+    assert (bt[0, :2] >= 0).all() and (bt[1] == -1).all() and (bt[2, :2] >= 0).all() and (bt[2, 2:] == -1).all()
+    with pytest.raises(RuntimeError, match="begin_step"):
+        c.append_kv_batch(0, torch.zeros(22, 2, 128), torch.zeros(22, 2, 128))
+    assert c.end_step().tolist() == [19, 0, 17]
+    used = c.pages_used
+    with pytest.raises(RuntimeError, match="Out of KV pages"):
+        c.begin_chunk([a, b], [60, 96])
+    with pytest.raises(RuntimeError, match="max_blocks"):
+        c.begin_chunk([b], [97])
+    with pytest.raises(ValueError, match="once"):
+        c.begin_chunk([a, a], [1, 1])
+    with pytest.raises(ValueError, match="counts"):
+        c.begin_chunk([a, b], [1])
+    assert c.pages_used == used  # a refused chunk takes no page
+    with pytest.raises(RuntimeError, match="begin_chunk"):
+        c.append_qkv_batch(0, None, None, None, None, None)
+
+
+# ------------------------------------------------------------------ GPU
+@pytest.fixture(scope="module")
+def dev():
+    return torch.device("cuda", 0)
+
+
+def _check_attention(got, q, k, v, prefix, lens, p_dtype):
+    """got against attention of q over per-sequence k / v [B, KVH, T, D] (the
+    first `prefix` tokens are sequence 0's for all)."""
+    kp, vp = k[0, :, :prefix], v[0, :, :prefix]
+    args = (q.double(), kp, vp, prefix, k[:, :, prefix:], v[:, :, prefix:], [n - prefix for n in lens])
+    ref = shared_prefix_ref(*args)
+    bound = attention_bound(*args, None, ref, p_dtype, got.dtype)
+    err = (got.double() - ref).abs()
+    assert bool((err <= bound).all()), float((err / bound.clamp(min=1e-30)).max())
+
+
+def _gathered(c, layer, ids, width):
+    bt = c.get_block_table_tensor(ids).long().clamp(min=0)[:, : (width + 15) // 16]
+    out = []
+    for pool, s in ((c.k_pool, c.k_scale), (c.v_pool, c.v_scale)):
+        x = pool[layer][bt].float().double() * (s.double() if c.dtype == E4M3 else 1.0)
+        out.append(x.transpose(1, 2).reshape(len(ids), c.num_kv_heads, -1, c.head_dim))
+    return out
+
+
+@gpu
+@pytest.mark.parametrize("dtype,pool", [(torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16), (torch.float16, E4M3)])
+def test_prompt_then_forked_steps_together(dev, dtype, pool):
+    """A prompt appended in chunks with norms and rotation, forked four times,
+    then three steps: rotate + append + shared-prefix decode, each against 64
+    bits on what the cache holds."""
+    L, KVH, QH, D, P = 2, 4, 16, 128, 150
+    c = make(pages=64, seqs=6, blocks=16, device=str(dev), dtype=pool, layers=L, heads=KVH)
+    if pool == E4M3:
+        c.set_fp8_scales(0.02, 0.02)
+    g = torch.Generator(device=dev).manual_seed(3)
+    rnd = lambda *s: torch.randn(*s, generator=g, device=dev)  # noqa: E731
+    cos, sin = fk.rope_table(512, D, device=dev)
+    qw, kw = (1 + 0.2 * rnd(D)).to(dtype), (1 + 0.2 * rnd(D)).to(dtype)
+    a = c.allocate_sequence()
+    prompt = [(1.5 * rnd(P, QH + 2 * KVH, D)).to(dtype) for _ in range(L)]
+    cut = lambda x: (x[:, :QH], x[:, QH:QH + KVH], x[:, QH + KVH:])  # noqa: E731
+    for lo, hi in ((0, 70), (70, P)):
+        c.begin_chunk([a], [hi - lo])
+        for layer in range(L):
+            q, k, v = cut(prompt[layer][lo:hi])
+            k_out = torch.empty(hi - lo, KVH, D, dtype=dtype, device=dev)
+            q_out = c.append_qkv_batch(layer, q, k, v, cos, sin, q_weight=qw, k_weight=kw, k_out=k_out)
+            both = fk.qk_norm_rope(q, k, cos, sin, torch.arange(lo, hi, device=dev), q_weight=qw, k_weight=kw)
+            assert torch.equal(q_out, both[0]) and torch.equal(k_out, both[1])
+        c.end_step()
+    assert c.seq_len(a) == P
+    n = P // PAGE_SIZE * PAGE_SIZE
+    ids = [c.fork_sequence(a, n) for _ in range(4)]
+    ref_rows = norm_rope_ref(cut(prompt[1])[1], cos, sin, torch.arange(P, device=dev), kw)[0]
+    kk, _ = _gathered(c, 1, [ids[2]], n)
+    step = {torch.float16: 2 ** -10, torch.bfloat16: 2 ** -7, E4M3: 2 ** -3}[pool]
+    assert float((kk[0].transpose(0, 1) - ref_rows[:n]).abs().max()) <= step * float(ref_rows.abs().max())
+    for s in range(3):
+        bt, pos, lens = c.begin_step(ids)
+        shared = c.shared_prefix_pages(ids)
+        assert shared == n // PAGE_SIZE
+        for layer in range(L):
+            q, k, v = cut((1.5 * rnd(4, QH + 2 * KVH, D)).to(dtype))
+            qr = c.append_qkv_batch(layer, q, k, v, cos, sin, q_weight=qw, k_weight=kw)
+            kw8 = dict(scale_k=c.k_scale, scale_v=c.v_scale) if pool == E4M3 else {}
+            out = fk.paged_flash_decode_shared_prefix(qr, c.k_pool[layer], c.v_pool[layer], bt[0, :shared], n, bt[:, shared:],
+                                                      lens - n, PAGE_SIZE, **kw8)
+            ks, vs = _gathered(c, layer, ids, n + s + 1)
+            _check_attention(out, qr, ks, vs, n, lens.tolist(), torch.bfloat16 if pool == torch.bfloat16 else torch.float16)
+        c.end_step()
+    assert fk.read_status() == 0
+
+
+@gpu
+@pytest.mark.parametrize("graphed", [False, True])
+def test_inputs_written_right_before_the_call(dev, graphed):
+    """What precedes the call in the stream writes what it reads, its prefix
+    too: a torch op writes q and a prefix page, the append kernel the step's
+    token; 200 steps, each against the same decode after a synchronisation."""
+    B, QH, KVH, D, P = 6, 16, 4, 128, 1600
+    g = torch.Generator(device=dev).manual_seed(9)
+    n = P // 16
+    pages = n + 4 * B
+    kp = torch.randn(pages, KVH, 16, D, generator=g, device=dev).half()
+    vp = torch.randn(pages, KVH, 16, D, generator=g, device=dev).half()
+    table = torch.arange(n, dtype=torch.int32, device=dev)
+    bt = (n + torch.arange(4 * B, dtype=torch.int32, device=dev)).view(B, 4)
+    q = torch.zeros(B, QH, D, dtype=torch.float16, device=dev)
+    pos = torch.zeros(B, dtype=torch.int32, device=dev)
+    lens = torch.zeros(B, dtype=torch.int32, device=dev)
+    src = torch.randn(3, B, max(QH, KVH), D, generator=g, device=dev).half()
+    page = torch.zeros(1, dtype=torch.int64, device=dev)
+    fresh = torch.randn(2, 1, KVH, 16, D, generator=g, device=dev).half()
+    plen = torch.tensor([P - 3], dtype=torch.int32, device=dev)
+
+    def decode():
+        return fk.paged_flash_decode_shared_prefix(q, kp, vp, table, plen, bt, lens, 16)
+
+    def step():
+        kp.index_copy_(0, page, fresh[0])
+        vp.index_copy_(0, page, fresh[1])
+        q.copy_(src[0])
+        paged_kv_append(src[1][:, :KVH], src[2][:, :KVH], kp, vp, bt, pos)
+        torch.add(pos, 1, out=lens)
+        return decode()
+
+    step()
+    out = None
+    if graphed:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+    for i in range(200):
+        src.normal_(generator=g)
+        fresh.normal_(generator=g)
+        pos.fill_(i % 64)
+        page.fill_((7 * i) % n)
+        if graphed:
+            graph.replay()
+        else:
+            out = step()
+        got = out.clone()
+        torch.cuda.synchronize()
+        assert torch.equal(got, decode()), i
+    assert fk.read_status() == 0
+
+
+class _Module:
+    is_causal = True
+
+    def __init__(self, layer_idx):
+        self.layer_idx = layer_idx
+        self.num_key_value_groups = 4
+
+
+@gpu
+@pytest.mark.parametrize("pool", [torch.float16, E4M3])
+def test_paged_adapter_decodes_forked_sequences_behind_their_prefix(dev, pool, monkeypatch):
+    """Forked sequences through the adapter give what unforked copies of them
+    give, and only the forked ones take the shared path."""
+    from fasterkernels_b200.paged_attn import paged_adapter
+    B, L, P = 5, 2, 4400
+    calls = []
+    real = paged_adapter.paged_flash_decode_shared_prefix
+    monkeypatch.setattr(paged_adapter, "paged_flash_decode_shared_prefix", lambda *a, **k: calls.append(a[4]) or real(*a, **k))
+    outs, caches = [], []
+    for forked in (True, False):
+        c = make(pages=6 * 300, seqs=6, blocks=290, device=str(dev), dtype=pool, layers=L, heads=2)
+        if pool == E4M3:
+            c.set_fp8_scales(0.02, 0.02)
+        g = torch.Generator(device=dev).manual_seed(5)
+        k = torch.randn(L, 2, 2, P, 128, generator=g, device=dev).half()
+        n = P // 16 * 16
+        if forked:
+            a = c.allocate_sequence()
+            for layer in range(L):
+                c.write_prefill(a, layer, k[layer, 0], k[layer, 1])
+            ids = [c.fork_sequence(a, n) for _ in range(B)]
+        else:
+            ids = [c.allocate_sequence() for _ in range(B)]
+            for sid in ids:
+                for layer in range(L):
+                    c.write_prefill(sid, layer, k[layer, 0, :, :n], k[layer, 1, :, :n])
+        fk.set_paged_attention_cache(c, ids)
+        got = []
+        try:
+            for step in range(3):
+                for layer in range(L):
+                    q = torch.randn(B, 8, 1, 128, generator=g, device=dev).half()
+                    kv = torch.randn(2, B, 2, 1, 128, generator=g, device=dev).half()
+                    o, _ = fk.custom_paged_attention_forward(_Module(layer), q, kv[0], kv[1], None, 128 ** -0.5)
+                    assert o.shape == (B, 8, 1, 128)
+                    got.append((q.squeeze(2), layer, o.squeeze(2), [c.seq_len(s) + (layer < L - 1) for s in ids]))
+        finally:
+            fk.set_paged_attention_cache(None, [])
+        outs.append(got)
+        caches.append((c, ids, n))
+    assert calls == [n] * (3 * L)
+    for (q, layer, a, lens), (_, _, b, _) in zip(*outs):
+        c, ids, n = caches[0]
+        ks, vs = _gathered(c, layer, ids, n + 3)
+        for got in (a, b):
+            _check_attention(got, q, ks, vs, n, lens, torch.float16)

@@ -534,3 +534,42 @@ def test_hf_rotary_drop_in(dev, unsqueeze_dim, cos_batch):
         _inside(got.reshape(B * S, -1, D), ref, amp)
     with pytest.raises(ValueError, match="sequence length"):
         fk.custom_hf_apply_rotary_pos_emb(*args, cos[:, :3], sin[:, :3], unsqueeze_dim=unsqueeze_dim)
+
+
+@gpu
+def test_hf_rotary_drop_in_inside_a_random_weight_model(dev, monkeypatch):
+    """A small random-init Qwen3 whose layers rotate with the drop-in: same
+    logits as with transformers' own function (which rounds the two products
+    and their sum to f16 where the drop-in rounds once), prompt and steps."""
+    from transformers import DynamicCache, Qwen3Config, Qwen3ForCausalLM
+    from transformers.models.qwen3 import modeling_qwen3
+    cfg = Qwen3Config(vocab_size=512, hidden_size=256, intermediate_size=512, num_hidden_layers=2, num_attention_heads=4,
+                      num_key_value_heads=2, head_dim=128, max_position_embeddings=512)
+    torch.manual_seed(0)
+    model = Qwen3ForCausalLM(cfg).to(device=dev, dtype=torch.float16).eval()
+    prompt = torch.randint(0, 512, (2, 33), device=dev)
+    feed = torch.randint(0, 512, (3, 2, 1), device=dev)
+
+    def run():
+        cache, logits = DynamicCache(config=cfg), []
+        with torch.no_grad():
+            logits.append(model(input_ids=prompt, past_key_values=cache, use_cache=True).logits[:, -1].float())
+            for t in feed:
+                logits.append(model(input_ids=t, past_key_values=cache, use_cache=True).logits[:, -1].float())
+        return torch.stack(logits)
+
+    want, calls = run(), []
+    monkeypatch.setattr(modeling_qwen3, "apply_rotary_pos_emb",
+                        lambda *a, **k: calls.append(1) or fk.custom_hf_apply_rotary_pos_emb(*a, **k))
+    got = run()
+    assert len(calls) == 2 * 4
+    torch.testing.assert_close(got, want, atol=3e-2, rtol=3e-2)
+
+
+def test_custom_ops_declare_what_they_write():
+    ns = torch.ops.fasterkernels_b200
+    for name, mutated in (("qk_norm_rope", {"q_out", "k_out", "k_pool", "v_pool", "status"}),
+                          ("shared_prefix_decode", {"out"})):
+        schema = getattr(ns, name).default._schema
+        written = {a.name for a in schema.arguments if a.alias_info is not None and a.alias_info.is_write}
+        assert written == mutated, (name, written)
