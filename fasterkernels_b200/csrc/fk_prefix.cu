@@ -30,7 +30,8 @@
 // CTA is a segment whose (max, sum, O) goes to the workspace.  Planned on the
 // device from the prefix length.
 //
-// Warps: 0-3 and 4-7 softmax of stream 0 and 1, 8-11 load Q, K and V, 12 issues
+// Warps: 0-3 and 4-7 softmax of stream 0 and 1 (they load Q too), 8-11 load K
+// and V, 12 issues
 // the MMAs.  A tile that the tensor cores read with one
 // descriptor needs its 8-row groups evenly spaced, so a page is loaded as one
 // box per 128-byte half, straight into its 16 rows of that half.  Each loader
@@ -226,12 +227,16 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
   PShared<ST, RAW>& sh = *reinterpret_cast<PShared<ST, RAW>*>(smem_raw + C::TILES);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
+  if (warp == 1 && lane == 0) {  // not a loader: what follows the fetch in its warp waits for it
+    prefetch_tmap(&p.tk);
+    prefetch_tmap(&p.tv);
+  }
   if (tid == 0) {
     for (int i = 0; i < ST; ++i) {
       mbar_init(smem_u32(&sh.full[i]), 4);
       mbar_init(smem_u32(&sh.empty[i]), 1);
     }
-    mbar_init(smem_u32(&sh.qfull), 4);
+    mbar_init(smem_u32(&sh.qfull), SOFT_WARPS);
     mbar_init(smem_u32(&sh.qempty), 1);
     for (int i = 0; i < 4; ++i) {
       mbar_init(smem_u32(&sh.s[0][0] + i), 1);
@@ -247,10 +252,6 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
     sh.bad = 0;
   }
   if (warp == MMA_WARP) tmem_alloc(smem_u32(&sh.tmem), 512);
-  if (tid == LOAD_WARP * 32) {
-    prefetch_tmap(&p.tk);
-    prefetch_tmap(&p.tv);
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -289,6 +290,9 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
     const float c = fmaxf(rsqrtf(static_cast<float>(D)) * LOG2E * fabsf(sk), 1e-30f);
     uint32_t sph = 0;  // parities of the two S buffers
     uint32_t oph = 0, dph = 0;  // parities of o (segments of more than one item) and done
+    uint32_t qph = 1;
+    const float sq = p.scale_q != nullptr ? __ldg(p.scale_q) : 1.f;
+    const uint32_t flip = sk < 0.f ? 0x80008000u : 0u;  // a negative scale turns Q over: the softmax sees |scale|
     bool alive = true;
     for (int g = g0; g < g1 && alive;) {
       PrefixSeg sg;
@@ -296,6 +300,60 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
       const int ni = sg.dual ? 2 * sg.tiles : sg.tiles;
       const int trow = (2 * sg.unit + (sg.dual ? s : 0)) * PROWS + row;
       const int tok00 = sg.t0 * PTOK + (sg.dual ? 0 : s * PITEM), tstep = sg.dual ? PITEM : PTOK;
+      // ---- Q: this stream's row tile (parity: the one tile, by stream 0), once
+      // the previous segment's products are done.  The softmax threads have
+      // nothing else to do yet, while a loader waits 2000 to 5000 cycles behind
+      // its first TMA (the tensor map is fetched then).
+      if (!(alive = wait(&sh.qempty, qph))) break;
+      qph ^= 1u;
+      if (sg.dual || s == 0) {
+        // Q of the MMA's type with aligned rows: all loads of the tile in flight
+        const bool q_plain = p.q_al16 != 0 && p.q_dtype == (MBF16 ? FK_DTYPE_BF16 : FK_DTYPE_F16) && flip == 0;
+        constexpr int CPR = D / 8, RPS = 128 / CPR;  // 16-byte chunks of a row, rows of a step
+        static_assert(RPS % 8 == 0, "the swizzle of row r0 + k RPS is that of row r0");
+        const int lt = tid & 127, ch = lt % CPR, r0 = lt / CPR;
+        // rows r0, r0 + RPS, ..: their element offsets go up by one step, and by
+        // one turn more where the step passes the end of a group
+        const int db = RPS / p.G, dg = RPS - db * p.G;
+        const long long step = db * p.q_b + dg * p.q_h, turn = p.q_b - p.G * p.q_h;
+        const int first = (2 * sg.unit + (sg.dual ? s : 0)) * PROWS + r0;
+        const int b = first / p.G;
+        int gg = first - b * p.G, left = p.rows - first;
+        long long e = b * p.q_b + (sg.h * p.G + gg) * p.q_h + ch * 8;
+        const uint32_t dst = sQ + s * C::TILE_BYTES + (ch >> 3) * HALF_BYTES + r0 * 128 +
+                             (static_cast<uint32_t>((ch & 7) ^ (r0 & 7)) << 4);
+        auto advance_row = [&]() {
+          left -= RPS;
+          e += step;
+          if ((gg += dg) >= p.G) {
+            gg -= p.G;
+            e += turn;
+          }
+        };
+        const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+        if (q_plain) {
+          uint4 x[PROWS / RPS];
+#pragma unroll
+          for (int k = 0; k < PROWS / RPS; ++k, advance_row()) {
+            x[k] = none;
+            if (left > 0) x[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(p.q) + e));
+          }
+#pragma unroll
+          for (int k = 0; k < PROWS / RPS; ++k) sts128(dst + k * RPS * 128, x[k].x, x[k].y, x[k].z, x[k].w);
+        } else {
+#pragma unroll 1
+          for (int k0 = 0; k0 < PROWS / RPS; k0 += 4) {
+            uint4 x[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k, advance_row()) x[k] = left > 0 ? load_q8<MBF16>(p, e, sq, flip) : none;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sts128(dst + (k0 + k) * RPS * 128, x[k].x, x[k].y, x[k].z, x[k].w);
+          }
+        }
+        fence_async_proxy();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.qfull));
       float m = NEG_INF, l = 0.f;
       for (int j = 0; j < ni; ++j) {
         const int buf = j & 1;
@@ -429,9 +487,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
     // ============================================================ loaders
     const int lw = warp - LOAD_WARP, lt = tid - LOAD_WARP * 32;
     int stage = 0;
-    uint32_t eph = 1, qph = 1;
-    const float sq = p.scale_q != nullptr ? __ldg(p.scale_q) : 1.f;
-    const uint32_t flip = sk < 0.f ? 0x80008000u : 0u;  // a negative scale turns Q over: the softmax sees |scale|
+    uint32_t eph = 1;
     bool alive = true;
     bool withhold = p.inject == 1;
     uint32_t raw_par = 0;  // parity of each raw slot's next completion
@@ -457,50 +513,6 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
       bool is_v;
       int tile = sg.t0 + load_item(0, sg.tiles, sg.dual, &is_v);
       int ent = lookup(tile);
-      // ---- Q: the unit's row tiles, behind the request of the first tile and
-      // once the previous segment's products are done
-      auto load_q = [&]() -> bool {
-        if (!wait(&sh.qempty, qph)) return false;
-        qph ^= 1u;
-        // Q of the MMA's type with aligned rows is copied asynchronously
-        const bool q_async = p.q_al16 != 0 && p.q_dtype == (MBF16 ? FK_DTYPE_BF16 : FK_DTYPE_F16) && flip == 0;
-        constexpr int CPR = D / 8, RPS = 128 / CPR;  // 16-byte chunks of a row, rows of a step
-        const int ch = lt % CPR;
-        const int db = RPS / p.G, dg = RPS - db * p.G;  // a step in sequences and group members
-#pragma unroll 1
-        for (int s = 0; s < (sg.dual ? 2 : 1); ++s) {
-          const uint32_t dst = sQ + s * C::TILE_BYTES + (ch >> 3) * HALF_BYTES;
-          int grow = (2 * sg.unit + s) * PROWS + lt / CPR;
-          int b = grow / p.G, gg = grow - b * p.G;
-#pragma unroll 8
-          for (int k = 0; k < PROWS / RPS; ++k) {
-            const int r = lt / CPR + k * RPS;
-            const long long e = b * p.q_b + (sg.h * p.G + gg) * p.q_h + ch * 8;
-            const uint32_t d = dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
-            const bool in = grow < p.rows;
-            if (q_async) {
-              cp_async16_zfill(d, static_cast<const unsigned short*>(p.q) + (in ? e : 0), in);
-            } else {
-              const uint4 x = in ? load_q8<MBF16>(p, e, sq, flip) : make_uint4(0u, 0u, 0u, 0u);
-              sts128(d, x.x, x.y, x.z, x.w);
-            }
-            grow += RPS;
-            b += db;
-            gg += dg;
-            if (gg >= p.G) {
-              gg -= p.G;
-              ++b;
-            }
-          }
-        }
-        cp_async_commit();
-        cp_async_wait<0>();
-        fence_async_proxy();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh.qfull));
-        return true;
-      };
-
       // ---- K and V tiles
       if constexpr (!FP8) {
         for (int idx = 0; idx < items; ++idx) {
@@ -552,7 +564,6 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
             if (lane == 0) mbar_arrive(full);
           }
           advance();
-          if (idx == 0 && !(alive = load_q())) break;
         }
       } else {
         // e4m3: raw pages RAW - 1 tiles ahead; this warp widens its own 32 rows
@@ -587,7 +598,6 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
 #pragma unroll
         for (int i = 0; i < RAW - 1; ++i)
           if (req < items) request(i);
-        alive = load_q();
         for (int i0 = 0; i0 < items && alive; i0 += RAW) {
 #pragma unroll
           for (int sl = 0; sl < RAW; ++sl) {
