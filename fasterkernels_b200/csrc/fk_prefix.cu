@@ -52,9 +52,6 @@
 
 namespace fk {
 
-#ifndef PSHARE
-#define PSHARE 1
-#endif
 constexpr int SOFT_WARPS = 8;  // warps 0-7: softmax; 8-11 loaders; 12 MMA issue
 constexpr int LOAD_WARP = SOFT_WARPS, MMA_WARP = SOFT_WARPS + 4;
 constexpr int PTHREADS = (MMA_WARP + 1) * 32;
@@ -63,6 +60,9 @@ constexpr int PTOK = 128;     // tokens of a token tile (a K or V tile in shared
 constexpr int PITEM = 64;     // tokens of an item (MMA N of QK, K of PV): half a tile
 constexpr int PPAGES = PTOK / PAGE;
 constexpr int HALF_BYTES = PTOK * 128;  // 128 rows of a 128-byte half
+// Of eight pairs of exponentials, those computed on the FMA units: measured 0:
+// 305 us, 1: 301, 2: 304 for the long case below, equal for the others.
+constexpr int FMA_PAIRS = 1;
 
 template <int KV, int D>
 struct PCfg {
@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
         }
         const float mb = (m == NEG_INF ? 0.f : m) - BIAS;
         // ---- P = 2^(x - m + BIAS).  Special-function units give 16 exponentials
-        // a cycle and SM, as many as the tensor cores take; some pairs are
+        // a cycle and SM, as many as the tensor cores take; one pair of eight is
         // computed on the FMA units instead.
         const f2 c2 = mk2(c, c), mb2 = mk2(-mb, -mb);
         f2 l0 = mk2(0.f, 0.f), l1 = mk2(0.f, 0.f);
@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
           for (int k = 0; k < 16; ++k) {
             f2 x = fma2(mk2(__uint_as_float(r[ch][2 * k]), __uint_as_float(r[ch][2 * k + 1])), c2, mb2);
             float p0, p1;
-            if (PSHARE > 0 && k % 8 < PSHARE) {
+            if (k % 8 < FMA_PAIRS) {
               x = exp2_fma(x);
               split2(x, p0, p1);
             } else {
@@ -835,7 +835,7 @@ __global__ void __launch_bounds__(JTHREADS) join_kernel(const __grid_constant__ 
     constexpr int N = decltype(count)::value;
     float Mn = M;
 #pragma unroll
-    for (int k = 0; k < N; ++k) Mn = fmaxf(Mn, ml[k].x);
+    for (int k = 0; k < N; ++k) Mn = max3_nan(Mn, ml[k].x, ml[k].x);
     if (Mn == NEG_INF) return;
     const float sc = exp2f(M - Mn);
     L *= sc;
@@ -877,6 +877,7 @@ __global__ void __launch_bounds__(JTHREADS) join_kernel(const __grid_constant__ 
       const bool ok = i + k < own.y;
       const long long rec = (oitem + own.x + i + k) * p.own.slots + slot;
       ml[k] = ok ? __ldcg(p.own.ml + rec) : none;
+      if (ml[k].y != ml[k].y) ml[k].x = ml[k].y;  // the own part's maximum passes NaN by, its sum does not
       av[k] = ok ? __ldcg(reinterpret_cast<const float4*>(p.own.acc + rec * HEAD_DIM + d0)) : zero;
     }
     merge(ml, av, std::integral_constant<int, JOWN>{});

@@ -166,6 +166,33 @@ def test_nothing_to_attend_and_empty_parts(dev):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,pool", [(torch.float16, None), (torch.bfloat16, None), (torch.float16, E4M3)])
+@pytest.mark.parametrize("P,lens", [(200, [40, 0, 70]), (0, [40, 33, 70]), (200, [0, 0, 0])])
+def test_a_nan_reaches_the_rows_that_attend_it_and_no_others(dev, dtype, pool, P, lens):
+    c = make(dev, P, lens, 8, 2, dtype=dtype, pool=pool, seed=6)
+    clean = call(c)
+    assert not bool(clean.isnan().any())
+    c["q"][0, 1, 5] = float("nan")
+    c["q"][1, 7, 0] = float("nan")
+    out = call(c)
+    hit = torch.zeros(3, 8, dtype=torch.bool, device=dev)
+    hit[0, 1] = hit[1, 7] = True
+    assert bool(out[hit].isnan().all()) and torch.equal(out[~hit], clean[~hit])
+    c = make(dev, P, lens, 8, 2, dtype=dtype, pool=pool, seed=6)
+    hit[:] = False
+    for row, page in ((slice(None), c["table"]), (2, c["bt"][2])):  # a K row of head 1: in the prefix, in sequence 2
+        if page.numel():
+            page = int(page[0])
+            if pool == E4M3:
+                c["k"].view(torch.uint8)[page, 1, 3] = 0x7f
+            else:
+                c["k"][page, 1, 3, 9] = float("nan")
+            hit[row, 4:] = True
+            out = call(c)
+            assert bool(out[hit].isnan().all()) and torch.equal(out[~hit], clean[~hit])
+
+
+@gpu
 def test_prefix_length_on_the_host_and_on_the_device(dev):
     c = make(dev, 700, [20, 5], 8, 2, seed=6)
     want = call(c)
