@@ -615,10 +615,11 @@ cudaError_t launch_rope(const fk_rope_args& a, int device, cudaStream_t stream) 
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms[device], cudaDevAttrMultiProcessorCount, device);
     if (e != cudaSuccess) return e;
   }
-  int fit = 0;  // blocks that share an SM
-  if (smem <= RS_MAX_SMEM)
+  const long long work = (a.tokens + tok - 1) / tok;
+  int fit = 0;  // blocks that share an SM (not asked for where one on each is too many already)
+  if (smem <= RS_MAX_SMEM && work >= 2 * sms[device])
     cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, rope_stream_kernel<D, POOL, IL, BF>, threads, static_cast<size_t>(smem));
-  const long long grid = static_cast<long long>(sms[device]) * fit, work = (a.tokens + tok - 1) / tok;
+  const long long grid = static_cast<long long>(sms[device]) * fit;
   // With fewer than two stages a block there is nothing to stream ahead; a
   // token too wide for the ring takes the same way.
   if (work < 2 * grid || fit == 0 || a.tokens > 0x7fe00000)
