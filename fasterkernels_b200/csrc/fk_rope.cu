@@ -26,8 +26,9 @@
 // append below).
 // Measured (device time, inputs past L2): 16384 tokens x 40 heads x 128 bf16
 // 61 us = 5.6 TB/s (86 % of the copy rate), 116 us with rope_step_kernel; the
-// same with v into bf16 pages 76 us = 5.4 TB/s; a step of 32 tokens 2.8 us, 3.9
-// us with rope_stream_kernel.
+// same with v into bf16 pages 76 us = 5.4 TB/s; 6007 x (24 + 4 + 4) heads into
+// e4m3 pages 19.3 us = 4.9 TB/s; a step of 32 tokens 2.8 us, 3.9 us with
+// rope_stream_kernel.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -71,15 +72,56 @@ __device__ __forceinline__ uint2 narrow4(const f2 (&x)[2]) {
   return make_uint2(w[0], w[1]);
 }
 
-// x / scale saturated to +-448, rounded to nearest e4m3 (a true division, as
-// fk_paged_kv_append)
-__device__ __forceinline__ uint32_t quant4(const f2 (&x)[2], float scale) {
-  uint32_t w = 0;
+// x / scale saturated to +-448, rounded to nearest e4m3, with the bits that a
+// true division gives (as fk_paged_kv_append), nearly always without one: the
+// rounded quotient lies between x * lo and x * hi, whose factors are the
+// reciprocal made 2^-21 smaller and larger (each of the three roundings on the
+// way, and the quotient's own, is off by 2^-24 at most), and rounding to e4m3 is
+// monotonic, so where the two ends agree that is the result.  Else (a quotient
+// next to the middle of two e4m3 values: 5e-6 of random ones) it divides.  By a
+// power of two the product is exact, ties included.  (Dividing always: 23.7
+// instead of 19.3 us for 6007 tokens x 32 heads, the k and v warps being late.)
+struct Quant {
+  float lo, hi;
+};
+__device__ __forceinline__ float quant_scale(const fk_rope_args& p, int kd) {
+  const float* sc = static_cast<const float*>(kd == 1 ? p.scale_k : p.scale_v);
+  return sc != nullptr ? __ldg(sc) : 1.f;
+}
+__device__ __forceinline__ Quant make_quant(const fk_rope_args& p, int kd) {
+  const float scale = quant_scale(p, kd);
+  const float a = fabsf(scale), r = 1.f / scale;
+  const bool pow2 = (__float_as_uint(scale) & 0x7fffffu) == 0;
+  Quant q = {pow2 ? r : r * 0.99999952316284f, pow2 ? r : r * 1.00000047683716f};
+  if (!(a >= 0x1p-100f && a <= 0x1p100f)) q.lo = -1.f, q.hi = 1.f;  // the reciprocal may leave f32's range: divide
+  return q;
+}
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3));
+}
+__device__ __forceinline__ uint2 quant8(const f2 (&x)[4], const Quant& q, const fk_rope_args& p, int kd) {
+  uint32_t a[4], b[4];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < 4; ++i) {
     float lo, hi;
-    split2(x[i], lo, hi);
-    w |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(lo / scale, hi / scale), __NV_SATFINITE, __NV_E4M3)) << (16 * i);
+    split2(mul2(x[i], mk2(q.lo, q.lo)), lo, hi);
+    a[i] = e4m3x2(lo, hi);
+    split2(mul2(x[i], mk2(q.hi, q.hi)), lo, hi);
+    b[i] = e4m3x2(lo, hi);
+  }
+  uint2 w = make_uint2(a[0] | (a[1] << 16), a[2] | (a[3] << 16));
+  if (w.x != (b[0] | (b[1] << 16)) || w.y != (b[2] | (b[3] << 16))) {
+    const float scale = quant_scale(p, kd);  // again: registers are short where this is seldom needed
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i) {
+      float lo, hi;
+      split2(i == 0 ? x[0] : i == 1 ? x[1] : i == 2 ? x[2] : x[3], lo, hi);
+      const uint32_t d = e4m3x2(lo / scale, hi / scale);
+      if (i == 0) w.x = d;
+      else if (i == 1) w.x |= d << 16;
+      else if (i == 2) w.y = d;
+      else w.y |= d << 16;
+    }
   }
   return w;
 }
@@ -112,10 +154,6 @@ __device__ __forceinline__ uint4 narrow8(const f2 (&x)[4]) {
   const f2 lo[2] = {x[0], x[1]}, hi[2] = {x[2], x[3]};
   const uint2 a = narrow4<BF>(lo), b = narrow4<BF>(hi);
   return make_uint4(a.x, a.y, b.x, b.y);
-}
-__device__ __forceinline__ uint2 quant8(const f2 (&x)[4], float scale) {
-  const f2 lo[2] = {x[0], x[1]}, hi[2] = {x[2], x[3]};
-  return make_uint2(quant4(lo, scale), quant4(hi, scale));
 }
 __device__ __forceinline__ void load8(const void* base, long long i, int dt, f2 (&x)[4]) {
   f2 t[2];
@@ -188,8 +226,7 @@ __device__ __forceinline__ void rope_turn(f2 (&xa)[4], f2 (&xb)[4], const f2 (&c
 // Store the lane's part: q / k to the dense output, k / v to the page slot.
 template <int POOL, bool BF>
 __device__ __forceinline__ void rope_store(const fk_rope_args& p, const f2 (&xa)[4], const f2 (&xb)[4], uint4 ra, uint4 rb,
-                                           int kd, int head, long long t, int phys, int slot, float sk, float sv, int da,
-                                           int db) {
+                                           int kd, int head, long long t, int phys, int slot, const Quant& qu, int da, int db) {
   if (kd == 0 || (kd == 1 && p.k_out != nullptr)) {
     unsigned short* dst = kd == 0 ? static_cast<unsigned short*>(p.q_out) + t * p.qo_t + head * p.qo_h
                                   : static_cast<unsigned short*>(p.k_out) + t * p.ko_t + head * p.ko_h;
@@ -200,9 +237,8 @@ __device__ __forceinline__ void rope_store(const fk_rope_args& p, const f2 (&xa)
   const long long o = kd == 1 ? phys * p.kp_p + slot * p.kp_s + head * p.kp_h : phys * p.vp_p + slot * p.vp_s + head * p.vp_h;
   if constexpr (POOL == 2) {
     unsigned char* dst = static_cast<unsigned char*>(kd == 1 ? p.k_pool : p.v_pool) + o;
-    const float sc = kd == 1 ? sk : sv;
-    *reinterpret_cast<uint2*>(dst + da) = quant8(xa, sc);
-    *reinterpret_cast<uint2*>(dst + db) = quant8(xb, sc);
+    *reinterpret_cast<uint2*>(dst + da) = quant8(xa, qu, p, kd);
+    *reinterpret_cast<uint2*>(dst + db) = quant8(xb, qu, p, kd);
   } else {
     unsigned short* dst = static_cast<unsigned short*>(kd == 1 ? p.k_pool : p.v_pool) + o;
     *reinterpret_cast<uint4*>(dst + da) = kd == 1 ? narrow8<BF>(xa) : ra;
@@ -289,8 +325,8 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_step_kernel(const __grid_co
     load8(w, db, wt, wb);
   }
   if (threadIdx.x == 0 && blockIdx.y == 0) rope_report<POOL>(p, pos_ok, phys);
-  const float sk = POOL == 2 && p.scale_k != nullptr ? __ldg(static_cast<const float*>(p.scale_k)) : 1.f;
-  const float sv = POOL == 2 && p.scale_v != nullptr ? __ldg(static_cast<const float*>(p.scale_v)) : 1.f;
+  Quant qu = {};
+  if (POOL == 2) qu = make_quant(p, kd);
   if (!pos_ok) {  // uniform
     rope_zero(p, kd, head, t, da, db);
     return;
@@ -304,7 +340,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_step_kernel(const __grid_co
       w1 = i < 4 ? wa[i + 1] : wb[i - 3];
     });
   if (rot && kd < 2) rope_turn<IL>(xa, xb, c, s);
-  if (kd < 3) rope_store<POOL, BF>(p, xa, xb, ra, rb, kd, head, t, phys, pos & 15, sk, sv, da, db);
+  if (kd < 3) rope_store<POOL, BF>(p, xa, xb, ra, rb, kd, head, t, phys, pos & 15, qu, da, db);
 }
 
 // ------------------------------------------------------------------------
@@ -474,8 +510,6 @@ __global__ void __launch_bounds__(RS_THREADS, 2) rope_stream_kernel(const __grid
   const int da = (!IL && rot) ? 8 * l : 16 * l;
   const int db = (!IL && rot) ? R / 2 + 8 * l : da + 8;
   const float eps = static_cast<float>(p.eps);
-  const float sk = POOL == 2 && p.scale_k != nullptr ? __ldg(static_cast<const float*>(p.scale_k)) : 1.f;
-  const float sv = POOL == 2 && p.scale_v != nullptr ? __ldg(static_cast<const float*>(p.scale_v)) : 1.f;
   const int tdt = static_cast<int>(p.table_dtype);
   const int tw = warp / sp.wpt, gw = warp - tw * sp.wpt;
   const int gpt = (rows + RPW - 1) / RPW;
@@ -489,6 +523,7 @@ __global__ void __launch_bounds__(RS_THREADS, 2) rope_stream_kernel(const __grid
   char* page = nullptr;             // row of slot 0 of page 0 in its pool, or null
   bool norm = false;
   uint32_t wts = 0;                 // its weights
+  Quant qu = {};
   auto row = [&](int g) {
     const int r = g * RPW + lane / LPH;
     int head;
@@ -507,6 +542,7 @@ __global__ void __launch_bounds__(RS_THREADS, 2) rope_stream_kernel(const __grid
     if (POOL && kd == 2) page = static_cast<char*>(p.v_pool) + head * p.vp_h * (POOL == 2 ? 1 : 2);
     norm = kd == 0 ? nq : kd == 1 && nk;
     wts = smem_u32(s_w[kd == 0 ? 0 : 1]);
+    if (POOL == 2) qu = make_quant(p, kd);
   };
   row(gw);
   int stage = 0;
@@ -567,9 +603,8 @@ __global__ void __launch_bounds__(RS_THREADS, 2) rope_stream_kernel(const __grid
           const long long at = kd == 1 ? s_tok[stage][j].k : s_tok[stage][j].v;
           if (at >= 0) {
             if constexpr (POOL == 2) {
-              const float sc = kd == 1 ? sk : sv;
-              *reinterpret_cast<uint2*>(page + at + da) = quant8(xa, sc);
-              *reinterpret_cast<uint2*>(page + at + db) = quant8(xb, sc);
+              *reinterpret_cast<uint2*>(page + at + da) = quant8(xa, qu, p, kd);
+              *reinterpret_cast<uint2*>(page + at + db) = quant8(xb, qu, p, kd);
             } else if (kd == 1) {
               *reinterpret_cast<uint4*>(page + 2 * (at + da)) = narrow8<BF>(xa);
               *reinterpret_cast<uint4*>(page + 2 * (at + db)) = narrow8<BF>(xb);
@@ -592,22 +627,18 @@ __global__ void __launch_bounds__(RS_THREADS, 2) rope_stream_kernel(const __grid
 
 constexpr int RS_MAX_SMEM = 200 * 1024;
 constexpr int RS_STAGE_BYTES = 26 * 1024;  // tokens are gathered up to this
+constexpr int RS_MIN_STAGES = 3;           // of a block (fewer: rope_step_kernel)
 
 template <int D, int POOL, bool IL, bool BF>
 cudaError_t launch_rope(const fk_rope_args& a, int device, cudaStream_t stream) {
   const long long rows = a.q_heads + (POOL ? 2 : 1) * a.kv_heads;
   const int table_bytes = static_cast<int>(a.rotary_dim / 2 * (a.table_dtype == FK_DTYPE_F32 ? 4 : 2));
   const long long tok_bytes = (rows * D * 2 + 2 * table_bytes + 127) / 128 * 128;
-  int tok = 1;
-  while (tok < RS_TOK && 2 * tok * tok_bytes <= RS_STAGE_BYTES) tok *= 2;
-  const long long smem = RS_STAGES * tok * tok_bytes;
   constexpr int HPP = ROPE_THREADS / (D / 16);
-  // Warps of a token: its groups of rows in as few rounds as ten warps allow.
+  // Warps of a token: its groups of rows in as few rounds as RS_WARPS allow.
   const int gpt = static_cast<int>((rows + HPP / 4 - 1) / (HPP / 4));
   const int rounds = (gpt + RS_WARPS - 1) / RS_WARPS;
   const int wpt = (gpt + rounds - 1) / rounds;
-  const int tpw = RS_WARPS / wpt < tok ? RS_WARPS / wpt : tok;
-  const int threads = (wpt * tpw + 1) * 32;
   if (device < 0 || device >= 64) return cudaErrorInvalidDevice;
   static int sms[64] = {};
   if (sms[device] == 0) {
@@ -615,14 +646,28 @@ cudaError_t launch_rope(const fk_rope_args& a, int device, cudaStream_t stream) 
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms[device], cudaDevAttrMultiProcessorCount, device);
     if (e != cudaSuccess) return e;
   }
-  const long long work = (a.tokens + tok - 1) / tok;
-  int fit = 0;  // blocks that share an SM (not asked for where one on each is too many already)
-  if (smem <= RS_MAX_SMEM && work >= 2 * sms[device])
+  // A block wants some stages to stream: stages of as many tokens as fit, of
+  // fewer where that leaves blocks with less than RS_MIN_STAGES.  (4099 tokens x
+  // 15 heads x 64: 6.2 us so, 8.2 with rope_step_kernel, which 26 KB stages and
+  // two of them a block would choose; 1200 x 40 x 128: 7.2 us, 7.8 with two.  With
+  // one, 300 x 48 x 128 takes 4.9 us, 3.8 with rope_step_kernel.)
+  int tok = 1, tpw = 1, threads = 0;
+  while (tok < RS_TOK && 2 * tok * tok_bytes <= RS_STAGE_BYTES) tok *= 2;
+  long long smem = 0, grid = 0, work = 0;
+  bool stream_ok = false;
+  for (; tok >= 1 && !stream_ok && a.tokens <= 0x7fe00000; tok /= 2) {
+    smem = RS_STAGES * tok * tok_bytes;
+    work = (a.tokens + tok - 1) / tok;
+    if (smem > RS_MAX_SMEM || work < 2 * sms[device]) continue;
+    tpw = RS_WARPS / wpt < tok ? RS_WARPS / wpt : tok;
+    threads = (wpt * tpw + 1) * 32;
+    int fit = 0;  // blocks that share an SM
     cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, rope_stream_kernel<D, POOL, IL, BF>, threads, static_cast<size_t>(smem));
-  const long long grid = static_cast<long long>(sms[device]) * fit;
-  // With fewer than two stages a block there is nothing to stream ahead; a
-  // token too wide for the ring takes the same way.
-  if (work < 2 * grid || fit == 0 || a.tokens > 0x7fe00000)
+    grid = static_cast<long long>(sms[device]) * fit;
+    stream_ok = fit > 0 && work >= RS_MIN_STAGES * grid;
+    if (stream_ok) break;
+  }
+  if (!stream_ok)
     return launch_pdl(rope_step_kernel<D, POOL, IL, BF>,
                       dim3(static_cast<unsigned>(a.tokens), static_cast<unsigned>((rows + HPP - 1) / HPP)),
                       dim3(ROPE_THREADS), 0, stream, a);

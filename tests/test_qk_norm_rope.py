@@ -387,6 +387,29 @@ def test_append_rope_without_rotation_equals_paged_kv_append(dev, pool):
 
 
 @gpu
+@pytest.mark.parametrize("T", [64, 4096])
+@pytest.mark.parametrize("scale", [1.0, 0.25, 1.5, 3.0, 0.0125, 0.7071, -0.3, 1e-33, 3e-39, 1e33, 0.0, float("inf")])
+def test_append_rope_quantises_every_value_as_a_division_does(dev, T, scale):
+    KVH, D = 8, 128
+    every = torch.arange(65536, dtype=torch.int32, device=dev).to(torch.int16).view(torch.bfloat16).view(64, KVH, D)
+    v = every.repeat(T // 64, 1, 1)
+    k = torch.zeros_like(v)
+    P = T // 16
+    bt = torch.arange(P, dtype=torch.int32, device=dev)[None]
+    pos, seq = torch.arange(T, dtype=torch.int32, device=dev), torch.zeros(T, dtype=torch.int32, device=dev)
+    pools = [torch.zeros(P, KVH, 16, D, device=dev).to(E4M3) for _ in range(4)]
+    s = torch.tensor(scale, device=dev)
+    fk.paged_kv_append_rope(k[:, :1], k, v, pools[0], pools[1], bt, pos, None, None, seq_ids=seq, scale_k=s, scale_v=s)
+    paged_kv_append(k, v, pools[2], pools[3], bt[0][:, None].repeat_interleave(16, 0), pos % 16, scale_k=s, scale_v=s)
+    assert torch.equal(pools[0].view(torch.uint8), pools[2].view(torch.uint8))
+    assert torch.equal(pools[1].view(torch.uint8), pools[3].view(torch.uint8))
+    # each quotient, rounded to f32 and to e4m3
+    want = (v.float() / s).clamp(-448, 448).to(E4M3).float()
+    got = pools[1].transpose(1, 2).reshape(T, KVH, D).float()
+    assert torch.equal(torch.nan_to_num(got, nan=1e4), torch.nan_to_num(want, nan=1e4))
+
+
+@gpu
 def test_append_rope_device_side_conditions(dev):
     q, k, v = _heads(dev, 7, 4, 2, 128, torch.float16, seed=8)
     cos, sin = fk.rope_table(50, 128, device=dev)
