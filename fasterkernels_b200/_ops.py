@@ -146,9 +146,9 @@ def rope_launch(q: torch.Tensor, k: torch.Tensor, v: Optional[torch.Tensor], cos
         kw = _WIDE_CODES[k_weight.dtype]
     if inner:
         args = _ROPE_ARGS.pack(
-            q.data_ptr(), k.data_ptr(), _addr(v), q_out.data_ptr(), _addr(k_out), _addr(k_pool), _addr(v_pool), _addr(cos),
-            _addr(sin), _addr(positions), _addr(seq_ids), _addr(bt), _addr(q_weight), _addr(k_weight), _addr(scale_k),
-            _addr(scale_v), _addr(status), q_t, q_h, k_t, k_h, v_t, v_h, qo_t, qo_h, ko_t, ko_h, kp_p, kp_h, kp_s, vp_p, vp_h,
+            *[0 if t is None else t.data_ptr()
+              for t in (q, k, v, q_out, k_out, k_pool, v_pool, cos, sin, positions, seq_ids, bt, q_weight, k_weight, scale_k,
+                        scale_v, status)], q_t, q_h, k_t, k_h, v_t, v_h, qo_t, qo_h, ko_t, ko_h, kp_p, kp_h, kp_s, vp_p, vp_h,
             vp_s, cos_row, sin_row, bt_b, T, QH, k.shape[1], D, 2 * R, interleaved, max_pos, bt_rows, blocks, pages,
             N.dtype_code(q.dtype), pool_code, table, qw, kw, eps)
         rc = N.lib().fk_qk_norm_rope(args, N.raw_stream(q.device.index))
@@ -165,7 +165,7 @@ def rope_launch(q: torch.Tensor, k: torch.Tensor, v: Optional[torch.Tensor], cos
 
 
 _PREFIX_ARGS = struct.Struct("13Q22q")  # fk_prefix_args of include/fk_decode.h
-_prefix_ws_bytes = {}
+_prefix_ws = {}
 
 
 def shared_prefix_launch(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, prefix_table: torch.Tensor,
@@ -180,24 +180,25 @@ def shared_prefix_launch(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     kv_code = N.dtype_code(k_pool.dtype)
     lib = N.lib()
     key = (dev.index, B, QH, KVH, D, kv_code)
-    need = _prefix_ws_bytes.get(key)
-    if need is None:
+    status = N.status_word(dev)
+    like = _prefix_ws.get(key)
+    if like is None:
         need = int(lib.fk_shared_prefix_workspace_bytes(*key))
         if need == 0:
             raise RuntimeError(f"fk_shared_prefix_workspace_bytes failed: {N.last_error()}")
-        _prefix_ws_bytes[key] = need
-    status = N.status_word(dev)
+        # a view without memory of its own: empty_like of it takes 1.4 us, empty 3.4
+        like = _prefix_ws[key] = status.view(torch.uint8)[:1].expand(need)
     # scratch of this call alone (torch's allocator reuses it in stream order;
     # in a captured graph it belongs to the graph's pool), so calls on other
     # streams and other graphs never share it
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    ws = torch.empty_like(like, memory_format=torch.contiguous_format)
     qs, ks, vs, os = q.stride(), k_pool.stride(), v_pool.stride(), out.stride()
     args = _PREFIX_ARGS.pack(
         q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), prefix_table.data_ptr(), _addr(prefix_len), bt.data_ptr(),
         lens.data_ptr(), _addr(s_aux), out.data_ptr(), _addr(scale_q), _addr(scale_k), _addr(scale_v), status.data_ptr(),
         prefix_len_host, prefix_table.shape[0], B, QH, KVH, D, P, bt.shape[1], N.dtype_code(q.dtype), kv_code,
         N.dtype_code(out.dtype), qs[0], qs[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], bt.stride(0), os[0], os[1])
-    N.check(lib.fk_paged_shared_prefix_decode(args, ws.data_ptr(), need, N.raw_stream(dev.index)),
+    N.check(lib.fk_paged_shared_prefix_decode(args, ws.data_ptr(), ws.numel(), N.raw_stream(dev.index)),
             "fk_paged_shared_prefix_decode")
 
 

@@ -100,7 +100,10 @@ def paged_flash_decode_shared_prefix(q, k_pool, v_pool, prefix_table, prefix_len
     sk = _scale_ptr(scale_k, dev) if e4m3 else None
     sv = _scale_ptr(scale_v, dev) if e4m3 else None
     if out is None:
-        out = torch.empty(B, QH, D, dtype=out_dtype, device=dev)
+        if q.dtype == out_dtype:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)  # 1.4 us; empty 3.4
+        else:
+            out = torch.empty(B, QH, D, dtype=out_dtype, device=dev)
     elif out.shape != (B, QH, D) or out.dtype != out_dtype or out.stride(-1) != 1 or out.device != dev:
         raise ValueError("out must be [B, Q_H, D] of out_dtype on q's device with unit inner stride")
     _ops.shared_prefix(q, k_pool, v_pool, prefix_table, prefix_len, host_len, bt, lens, s_aux, sq, sk, sv, out)

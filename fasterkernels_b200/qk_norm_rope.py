@@ -89,7 +89,7 @@ def _check_weight(w, name, D, dev):
 
 def _check_out(out, like, name):
     if out is None:
-        return like.new_empty(like.shape)
+        return torch.empty_like(like, memory_format=torch.contiguous_format)  # 1.4 us; new_empty 2.4, empty 3.4
     if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device or out.stride(-1) != 1:
         raise ValueError(f"{name} must have the shape, dtype and device of its input, with unit inner stride")
     return out
