@@ -21,18 +21,17 @@
 //   columns each): S of item j + 1 is there before the softmax of item j ends,
 //   so that it never waits for the chain P V, Q K^T.  (With 128-token items there
 //   is room for one S a stream, and that chain, 1100 cycles, was added to every
-//   tile: 395 us for the long case below.)  P (f16, or bf16 for bf16 KV)
+//   tile: 395 us instead of 319, at that time, for the long case below.)  P (f16, or bf16 for bf16 KV)
 //   overwrites half of its own S and is the A operand of O += P V from there.
 //
 // Work is cut like the decode kernel's: units (KV head, one or two row tiles)
 // laid end to end in granules (dual: one token tile, parity: two), each CTA of
 // the persistent grid takes an equal run of them, and the piece of a unit in a
 // CTA is a segment whose (max, sum, O) goes to the workspace.  Planned on the
-// device from the prefix length.
+// device from the prefix length and the own lengths.
 //
 // Warps: 0-3 and 4-7 softmax of stream 0 and 1 (they load Q too), 8-11 load K
-// and V, 12 issues
-// the MMAs.  A tile that the tensor cores read with one
+// and V, 12 issues the MMAs.  A tile that the tensor cores read with one
 // descriptor needs its 8-row groups evenly spaced, so a page is loaded as one
 // box per 128-byte half, straight into its 16 rows of that half.  Each loader
 // warp loads two of a tile's eight pages: one warp issues a box in 100 to 150
@@ -41,6 +40,18 @@
 // from there.  Tiles that end the prefix or hold a bad page are loaded row by
 // row instead, with zeros where there is no token (the tail of a page may hold
 // anything, and 0 x NaN would reach the output).
+//
+// Bound.  An item pair takes 1280 cycles of tensor work: Q K^T with N = 64 runs
+// at the rate of its shared-memory reads (48 cycles per MMA of 32: 4 KB of Q and 2
+// KB of K at 128 bytes a cycle), P V at the MMA rate.  Measured 1800 to 1950
+// cycles: the chain P ready -> P V, Q K^T issue -> S ready passes through one
+// issuing warp, and e4m3 widening takes 512 cycles of shared-memory bandwidth more.
+// Device times, own part and join included (B200): long case, 128 sequences x 64
+// heads (8 KV heads), 65536 tokens of e4m3 + tails up to 1000, 300 us = 0.92
+// PFLOP/s; 64 x 32 heads, 32768 tokens of f16 + tails up to 512, 70 us, of which
+// the own part's reads take 20 to 27 and the join 9; 2 x 32 heads, 131072 tokens of
+// bf16, 106 us = 5.1 TB/s; 4 x 32 heads, 1000 tokens, 16 us, three kernels'
+// latencies.
 #include <cuda_fp8.h>
 
 #include <type_traits>
@@ -63,6 +74,11 @@ constexpr int HALF_BYTES = PTOK * 128;  // 128 rows of a 128-byte half
 // Of eight pairs of exponentials, those computed on the FMA units: measured 0:
 // 305 us, 1: 301, 2: 304 for the long case below, equal for the others.
 constexpr int FMA_PAIRS = 1;
+// Granules that starting behind the own part costs a CTA.  16-bit, 32 x 8 heads,
+// 4096 tokens behind 16 tails of 20: 17.4 us with 64 CTAs of two granules, 23.2
+// with 128 of one, which the SMs beside the own part do not hold.  2 to 9
+// measured: from 4 on some calls lose (48 x 64 heads, 2048 tokens: 30 -> 43 us).
+constexpr int WAIT = 2;
 
 template <int KV, int D>
 struct PCfg {
@@ -80,6 +96,7 @@ struct PShared {
   uint64_t full[ST], empty[ST], qfull, qempty, s[2][2], p[2][2], o[2], done[2], drain;
   uint64_t raw[4][RAW];              // a loader warp's e4m3 pages
   uint32_t tmem;
+  int busy;                          // SMs at work on the own part
   volatile int bad;                  // a bad page was seen: the softmax checks pages from then on
 };
 template <int KV, int D>
@@ -103,6 +120,9 @@ struct PrefixParams {
   int rows, G, kv_heads, q_dtype, q_al16;
   const float* scale_q;
   const float* scale_k;
+  const int* seq_lens;  // of the own tokens: what keeps SMs from the prefix at first
+  int batch, own_items;
+  int* plan;            // granules of a CTA, for the join
   float2* ml;
   float* acc;
   int* status;          // or null
@@ -110,20 +130,29 @@ struct PrefixParams {
   int inject;
 };
 
-// Granules and units, from the prefix length (device side).  32-bit: the host
-// refuses more than 2^30 granules, and warps that gave their registers away
-// must not call the 64-bit division's slow path.
+// Granules and units, from the prefix length (device side).  In 32 bits: the
+// host refuses more than 2^30 granules.
 struct PrefixPlan {
   int nt, nd, upu;       // token tiles; dual units and units of a KV head
-  int gh, total, per;    // granules of a KV head, in all, of a CTA
-  __device__ PrefixPlan(int plen, int rows, int kv_heads, int ctas) {
+  int gh, total;         // granules of a KV head, in all
+  int per;               // of a CTA
+  __device__ PrefixPlan(int plen, int rows, int kv_heads) {
     const int rt = (rows + PROWS - 1) / PROWS;
     nt = (plen + PTOK - 1) / PTOK;
     nd = rt / 2;
     upu = nd + (rt & 1);
     gh = nd * nt + ((rt & 1) ? (nt + 1) / 2 : 0);
     total = gh * kv_heads;
+  }
+  // A CTA that finds its SM taken by the own part starts about as late as
+  // WAIT granules take, so with few granules a run that fits the other SMs'
+  // CTAs is the shorter way.
+  __device__ void cut(int ctas, int busy) {
     per = max((total + ctas - 1) / ctas, 1);
+    if (ctas > busy) {
+      const int few = (total + ctas - busy - 1) / (ctas - busy);
+      if (few - per <= WAIT) per = max(few, 1);
+    }
   }
   // First granule and length of unit u of a KV head.
   __device__ int unit_base(int u) const { return u * nt; }
@@ -227,6 +256,8 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
   PShared<ST, RAW>& sh = *reinterpret_cast<PShared<ST, RAW>*>(smem_raw + C::TILES);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
+  bool past;
+  const int plen = prefix_len(p.plen_dev, p.plen, p.blocks, &past);
   if (warp == 1 && lane == 0) {  // not a loader: what follows the fetch in its warp waits for it
     prefetch_tmap(&p.tk);
     prefetch_tmap(&p.tv);
@@ -252,6 +283,25 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
     sh.bad = 0;
   }
   if (warp == MMA_WARP) tmem_alloc(smem_u32(&sh.tmem), 512);
+  if (warp == 2) {
+    // SMs that the own part keeps busy, by its plan: equal runs of 16-token
+    // granules, MIN_PER at least, over its grid, whose CTAs go to SMs of their
+    // own first.  Only whether all are busy counts, so a prefix of the batch may do.
+    long long u = 0;
+    const long long all = static_cast<long long>(gridDim.x) * MIN_PER;
+    for (int b0 = 0; b0 < p.batch && u < all; b0 += 128) {
+      long long n = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int b = b0 + 32 * i + lane;
+        if (b < p.batch) n += (max(__ldg(p.seq_lens + b), 0) + 15ll) >> 4;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+      u += n * p.own_items;
+    }
+    if (lane == 0) sh.busy = static_cast<int>(min((u + MIN_PER - 1) / MIN_PER, static_cast<long long>(gridDim.x)));
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -263,10 +313,10 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
   // kernel start after their own wait for what precedes them.
   grid_dependency_trigger();
 
-  bool past;
-  const int plen = prefix_len(p.plen_dev, p.plen, p.blocks, &past);
   if (past && blockIdx.x == 0 && tid == 0 && p.status != nullptr) atomicOr(p.status, FK_STATUS_BAD_PAGE);
-  const PrefixPlan pl(plen, p.rows, p.kv_heads, gridDim.x);
+  PrefixPlan pl(plen, p.rows, p.kv_heads);
+  pl.cut(gridDim.x, sh.busy);
+  if (blockIdx.x == 0 && tid == 0) *p.plan = pl.per;
   const int g0 = min(static_cast<int>(blockIdx.x) * pl.per, pl.total), g1 = min(g0 + pl.per, pl.total);
   const float sk = (FP8 && p.scale_k != nullptr) ? __ldg(p.scale_k) : 1.f;
   auto timed_out = [&]() {
@@ -785,8 +835,9 @@ struct JoinParams {
   const float2* ml;       // prefix segments
   const float* acc;
   OwnRecords own;
+  const int* plan;        // granules of a prefix CTA
   const int* plen_dev;
-  int plen, blocks, rows, G, kv_heads, q_heads, ctas;
+  int plen, blocks, rows, G, kv_heads;
   const float* s_aux;
   const float* scale_v;
   void* out;
@@ -803,6 +854,7 @@ template <int D>
 __global__ void __launch_bounds__(JTHREADS) join_kernel(const __grid_constant__ JoinParams p) {
   grid_dependency_wait();
   grid_dependency_trigger();
+  const int per = __ldcg(p.plan);
   const int per_head = (p.rows + p.rb - 1) / p.rb;
   const int h = blockIdx.x / per_head, first = blockIdx.x % per_head * p.rb;  // the block's first row
   const int tile = first / PROWS, row = first % PROWS + (threadIdx.x & (p.rb - 1));
@@ -816,14 +868,14 @@ __global__ void __launch_bounds__(JTHREADS) join_kernel(const __grid_constant__ 
   const int2 own = __ldcg(p.own.info + oitem);  // needed last: the prefix's records are read meanwhile
   bool past;
   const int plen = prefix_len(p.plen_dev, p.plen, p.blocks, &past);
-  const PrefixPlan pl(plen, p.rows, p.kv_heads, p.ctas);
+  const PrefixPlan pl(plen, p.rows, p.kv_heads);
   const int unit = tile >> 1;
   const bool dual = unit < pl.nd;
   long long rec0 = 0;  // the row's records: every (dual) second one from rec0 on
   int nrec = 0;
   if (pl.nt > 0) {
     const int base = h * pl.gh + pl.unit_base(unit);
-    const int c0 = base / pl.per, c1 = (base + pl.unit_len(unit) - 1) / pl.per;
+    const int c0 = base / per, c1 = (base + pl.unit_len(unit) - 1) / per;
     rec0 = 2ll * (c0 + h * pl.upu + unit) + (dual ? (tile & 1) : 0);
     nrec = (c1 - c0 + 1) * (dual ? 1 : 2);
   }
@@ -916,9 +968,9 @@ int prefix_ctas(int device) {
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
-// [own part's decode workspace | its items' records | prefix (max, sum) | prefix acc]
+// [own part's decode workspace | its items' records | plan | prefix (max, sum) | prefix acc]
 struct PrefixWs {
-  size_t own, info, ml, acc, total;
+  size_t own, info, plan, ml, acc, total;
   PrefixWs(int device, int batch, int q_heads, int kv_heads, int head_dim, int kv_dtype) {
     own = fk_decode_workspace_bytes_gqa(device, batch, q_heads, kv_heads, kv_dtype);
     const long long rows = static_cast<long long>(batch) * (q_heads / kv_heads);
@@ -926,7 +978,8 @@ struct PrefixWs {
     const size_t segs = static_cast<size_t>(prefix_ctas(device)) + static_cast<size_t>(kv_heads) * ((rt + 1) / 2);
     const size_t items = static_cast<size_t>(batch) * q_heads;  // at most
     info = up256(own);
-    ml = up256(info + items * sizeof(int2));
+    plan = up256(info + items * sizeof(int2));
+    ml = plan + 256;
     acc = up256(ml + segs * 2 * PROWS * sizeof(float2));
     total = own == 0 ? 0 : up256(acc + segs * 2 * PROWS * head_dim * sizeof(float));
   }
@@ -1044,6 +1097,10 @@ extern "C" int fk_paged_shared_prefix_decode(const fk_prefix_args* a, void* work
   JoinParams j = {};
   rc = own_part_launch(own, reinterpret_cast<int2*>(ws + w.info), p.status, w.own, st, &j.own);
   if (rc != FK_OK) return rc;
+  p.seq_lens = static_cast<const int*>(a->seq_lens);
+  p.batch = B;
+  p.own_items = j.own.per_seq;
+  j.plan = p.plan = reinterpret_cast<int*>(ws + w.plan);
   if (kv == FK_DTYPE_F16) rc = D == 64 ? launch_prefix<FK_DTYPE_F16, 64>(p, ctas, device, st) : launch_prefix<FK_DTYPE_F16, 128>(p, ctas, device, st);
   else if (kv == FK_DTYPE_BF16) rc = D == 64 ? launch_prefix<FK_DTYPE_BF16, 64>(p, ctas, device, st) : launch_prefix<FK_DTYPE_BF16, 128>(p, ctas, device, st);
   else rc = launch_prefix<FK_DTYPE_E4M3, 128>(p, ctas, device, st);
@@ -1056,8 +1113,6 @@ extern "C" int fk_paged_shared_prefix_decode(const fk_prefix_args* a, void* work
   j.rows = p.rows;
   j.G = p.G;
   j.kv_heads = KVH;
-  j.q_heads = QH;
-  j.ctas = ctas;
   j.s_aux = static_cast<const float*>(a->s_aux);
   j.scale_v = kv == FK_DTYPE_E4M3 ? static_cast<const float*>(a->scale_v) : nullptr;
   j.out = a->out;
