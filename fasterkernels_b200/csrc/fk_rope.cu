@@ -25,8 +25,8 @@
 // registers for each spill or cost a block per SM (123 instead of 76 us for the
 // append below).
 // Measured (device time, inputs past L2): 16384 tokens x 40 heads x 128 bf16
-// 61 us = 5.6 TB/s (86 % of the copy rate), 116 us with rope_step_kernel; the
-// same with v into bf16 pages 76 us = 5.4 TB/s; 6007 x (24 + 4 + 4) heads into
+// 58.7 us = 5.9 TB/s (89 % of the copy rate), 116 us with rope_step_kernel; the
+// same with v into bf16 pages 72 us = 5.7 TB/s; 6007 x (24 + 4 + 4) heads into
 // e4m3 pages 19.3 us = 4.9 TB/s; a step of 32 tokens 2.8 us, 3.9 us with
 // rope_stream_kernel.
 #include <cuda_bf16.h>
@@ -380,7 +380,12 @@ __global__ void __launch_bounds__(RS_THREADS, 2) rope_stream_kernel(const __grid
   constexpr int RPW = 32 / LPH;  // head rows of a warp
   constexpr int ROWB = D * 2;
   extern __shared__ __align__(128) unsigned char ring[];
-  __shared__ float4 s_w[2][D / 4];  // norm weights of q and k
+  // Norm weights of q and k, as the lanes of a row read them: their first four
+  // dims side by side, their second four, ..  (With dims in order the lanes of a
+  // read are 32 bytes apart, two of them on each bank: 61.5 instead of 58.7 us for
+  // 16384 tokens x 40 heads.  The same for f32 angles, by reading the halves in
+  // turned order, costs selects and registers: 69 us.)
+  __shared__ float4 s_w[2][4][LPH];
   __shared__ __align__(8) uint64_t full[RS_STAGES], empty[RS_STAGES];
   __shared__ RopeTok s_tok[RS_STAGES][RS_TOK];
   __shared__ int s_pos[RS_STAGES][RS_TOK];
@@ -494,15 +499,17 @@ __global__ void __launch_bounds__(RS_THREADS, 2) rope_stream_kernel(const __grid
   // ---- workers: warp w takes the groups of RPW rows w % wpt, + wpt, .. of the
   // tokens w / wpt, + tpw, .. of a stage
   for (int i = threadIdx.x; i < 2 * (D / 4); i += workers * 32) {
-    const int j = i % (D / 4);
-    const void* w = i < D / 4 ? p.q_weight : p.k_weight;
+    const int kind = i / (D / 4), piece = i % (D / 4) / LPH, wl = i % LPH;
+    const void* w = kind == 0 ? p.q_weight : p.k_weight;
     if (w == nullptr) continue;
+    const bool turned = !IL && wl < R / 16;  // the dims of a lane: see da, db
+    const int at = (piece < 2 ? (turned ? 8 * wl : 16 * wl) : (turned ? R / 2 + 8 * wl : 16 * wl + 8)) + 4 * (piece & 1);
     f2 x[2];
-    load4(w, 4 * j, static_cast<int>(i < D / 4 ? p.q_weight_dtype : p.k_weight_dtype), x);
+    load4(w, at, static_cast<int>(kind == 0 ? p.q_weight_dtype : p.k_weight_dtype), x);
     float4 f;
     split2(x[0], f.x, f.y);
     split2(x[1], f.z, f.w);
-    s_w[i / (D / 4)][j] = f;
+    s_w[kind][piece][wl] = f;
   }
   named_bar_sync(1, workers * 32);
   const int l = lane & (LPH - 1);
@@ -541,7 +548,7 @@ __global__ void __launch_bounds__(RS_THREADS, 2) rope_stream_kernel(const __grid
     if (POOL && kd == 1) page = static_cast<char*>(p.k_pool) + head * p.kp_h * (POOL == 2 ? 1 : 2);
     if (POOL && kd == 2) page = static_cast<char*>(p.v_pool) + head * p.vp_h * (POOL == 2 ? 1 : 2);
     norm = kd == 0 ? nq : kd == 1 && nk;
-    wts = smem_u32(s_w[kd == 0 ? 0 : 1]);
+    wts = smem_u32(&s_w[kd == 0 ? 0 : 1][0][l]);
     if (POOL == 2) qu = make_quant(p, kd);
   };
   row(gw);
@@ -567,7 +574,7 @@ __global__ void __launch_bounds__(RS_THREADS, 2) rope_stream_kernel(const __grid
         widen8<BF>(lds128(base + off + db * 2), xb);
         if (nq || nk)  // uniform over the grid
           rope_norm<D>(xa, xb, norm, eps, [&](int i, f2& w0, f2& w1) {
-            const uint4 w = lds128(wts + (i < 4 ? da : db) * 4 + (i & 2) * 8);
+            const uint4 w = lds128(wts + (i / 2) * (LPH * 16));
             w0 = mk2(__uint_as_float(w.x), __uint_as_float(w.y));
             w1 = mk2(__uint_as_float(w.z), __uint_as_float(w.w));
           });
