@@ -336,8 +336,9 @@ __global__ void __launch_bounds__(PTHREADS, 1) prefix_kernel(const __grid_consta
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // lane (warp & 3) * 32 in bits 16..
     const uint32_t tO = tmem + lanes + 256 + s * D;
-    // never 0: a masked logit (-inf) stays one
-    const float c = fmaxf(rsqrtf(static_cast<float>(D)) * LOG2E * fabsf(sk), 1e-30f);
+    // never 0: a masked logit (-inf) stays one (and NaN stays NaN)
+    const float cs = rsqrtf(static_cast<float>(D)) * LOG2E * fabsf(sk);
+    const float c = cs < 1e-30f ? 1e-30f : cs;
     uint32_t sph = 0;  // parities of the two S buffers
     uint32_t oph = 0, dph = 0;  // parities of o (segments of more than one item) and done
     uint32_t qph = 1;

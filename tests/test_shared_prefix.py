@@ -193,6 +193,17 @@ def test_a_nan_reaches_the_rows_that_attend_it_and_no_others(dev, dtype, pool, P
 
 
 @gpu
+def test_scales_of_zero_and_nan(dev):
+    c = make(dev, 200, [0, 0], 8, 2, pool=E4M3, seed=7)
+    for k, v in ((0.0, 0.02), (0.02, 0.0)):
+        c["sk"], c["sv"] = torch.tensor(k, device=dev), torch.tensor(v, device=dev)
+        check(c, call(c))
+    for k, v in ((float("nan"), 0.02), (0.02, float("nan"))):
+        c["sk"], c["sv"] = torch.tensor(k, device=dev), torch.tensor(v, device=dev)
+        assert bool(call(c).isnan().all())
+
+
+@gpu
 def test_prefix_length_on_the_host_and_on_the_device(dev):
     c = make(dev, 700, [20, 5], 8, 2, seed=6)
     want = call(c)
