@@ -118,6 +118,7 @@ def rope_launch(q: torch.Tensor, k: torch.Tensor, v: Optional[torch.Tensor], cos
     T, QH, D = q.shape
     if T == 0:
         return
+    _, KH, _ = k.shape
     q_t, q_h, q_d = q.stride()
     k_t, k_h, k_d = k.stride()
     qo_t, qo_h, _ = q_out.stride()
@@ -138,7 +139,7 @@ def rope_launch(q: torch.Tensor, k: torch.Tensor, v: Optional[torch.Tensor], cos
         vp_p, vp_h, vp_s, _ = v_pool.stride()
         pool_code, pages = N.dtype_code(k_pool.dtype), k_pool.shape[0]
         bt_rows, blocks = bt.shape
-        bt_b = bt.stride(0)
+        bt_b, _ = bt.stride()
     qw = kw = 0
     if q_weight is not None:
         qw = _WIDE_CODES[q_weight.dtype]
@@ -149,7 +150,7 @@ def rope_launch(q: torch.Tensor, k: torch.Tensor, v: Optional[torch.Tensor], cos
             *[0 if t is None else t.data_ptr()
               for t in (q, k, v, q_out, k_out, k_pool, v_pool, cos, sin, positions, seq_ids, bt, q_weight, k_weight, scale_k,
                         scale_v, status)], q_t, q_h, k_t, k_h, v_t, v_h, qo_t, qo_h, ko_t, ko_h, kp_p, kp_h, kp_s, vp_p, vp_h,
-            vp_s, cos_row, sin_row, bt_b, T, QH, k.shape[1], D, 2 * R, interleaved, max_pos, bt_rows, blocks, pages,
+            vp_s, cos_row, sin_row, bt_b, T, QH, KH, D, 2 * R, interleaved, max_pos, bt_rows, blocks, pages,
             N.dtype_code(q.dtype), pool_code, table, qw, kw, eps)
         rc = N.lib().fk_qk_norm_rope(args, N.raw_stream(q.device.index))
         if rc == 0:
@@ -197,7 +198,7 @@ def shared_prefix_launch(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
         q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), prefix_table.data_ptr(), _addr(prefix_len), bt.data_ptr(),
         lens.data_ptr(), _addr(s_aux), out.data_ptr(), _addr(scale_q), _addr(scale_k), _addr(scale_v), status.data_ptr(),
         prefix_len_host, prefix_table.shape[0], B, QH, KVH, D, P, bt.shape[1], N.dtype_code(q.dtype), kv_code,
-        N.dtype_code(out.dtype), qs[0], qs[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], bt.stride(0), os[0], os[1])
+        N.dtype_code(out.dtype), qs[0], qs[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], bt.stride()[0], os[0], os[1])
     N.check(lib.fk_paged_shared_prefix_decode(args, ws.data_ptr(), ws.numel(), N.raw_stream(dev.index)),
             "fk_paged_shared_prefix_decode")
 

@@ -46,15 +46,15 @@ def paged_kv_append_rope(q, k, v, k_pool, v_pool, block_table, positions, cos, s
         raise ValueError("pools must be [num_pages, KV_H, 16, D] with the heads and head dim of k")
     if v_pool.dtype != pdt or k_pool.device != dev or v_pool.device != dev:
         raise ValueError("the pools must have one dtype and be on q's device")
-    if k_pool.stride(-1) != 1 or v_pool.stride(-1) != 1:
+    if k_pool.stride()[3] != 1 or v_pool.stride()[3] != 1:
         raise ValueError("the pools must have unit inner stride")
     pool_code = N.dtype_code(pdt)
     if pool_code != N.FK_DTYPE_E4M3 and pdt != dt:
         raise TypeError("a 16-bit pool must have the dtype of k and v")
-    if block_table.dim() != 2 or block_table.device != dev:
-        raise ValueError("block_table must be [B, max_blocks] on q's device")
     bt = block_table
-    if bt.dtype != torch.int32 or bt.stride(1) != 1:
+    if bt.dim() != 2 or bt.device != dev:
+        raise ValueError("block_table must be [B, max_blocks] on q's device")
+    if bt.dtype != torch.int32 or bt.stride()[1] != 1:
         bt = bt.to(torch.int32).contiguous()
     positions = _check_idx(positions, "positions", dev)
     if seq_ids is not None:

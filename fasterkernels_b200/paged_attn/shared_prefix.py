@@ -13,7 +13,7 @@ import torch
 
 from .. import _native as N
 from .. import _ops
-from ..gqa_decode import HEAD_DIMS, _check_idx, _check_sink, _inner_contig
+from ..gqa_decode import HEAD_DIMS, _check_idx, _check_sink
 from ..gqa_decode_hf import _scale_ptr
 
 
@@ -70,9 +70,12 @@ def paged_flash_decode_shared_prefix(q, k_pool, v_pool, prefix_table, prefix_len
         out_dtype = q.dtype if q.dtype != torch.float8_e4m3fn else torch.float16
     if out_dtype not in (torch.float16, torch.bfloat16):
         raise TypeError("out_dtype must be float16 or bfloat16")
-    q = _inner_contig(q, "q")
-    k_pool = _inner_contig(k_pool, "k_pool")
-    v_pool = _inner_contig(v_pool, "v_pool")
+    if q.stride()[2] != 1:
+        q = q.contiguous()
+    if k_pool.stride()[3] != 1:
+        k_pool = k_pool.contiguous()
+    if v_pool.stride()[3] != 1:
+        v_pool = v_pool.contiguous()
     if prefix_table.dim() != 1:
         raise ValueError("prefix_table must be [n]")
     prefix_table = _check_idx(prefix_table, "prefix_table", dev)
@@ -90,7 +93,7 @@ def paged_flash_decode_shared_prefix(q, k_pool, v_pool, prefix_table, prefix_len
     bt = block_table
     if bt.device != dev:
         raise ValueError("block_table must be on q's device")
-    if bt.dtype != torch.int32 or (bt.stride(1) != 1 and bt.shape[1] > 1):
+    if bt.dtype != torch.int32 or (bt.stride()[1] != 1 and bt.shape[1] > 1):
         bt = bt.to(torch.int32).contiguous()
     lens = _check_idx(seq_lens, "seq_lens", dev)
     if lens.numel() < B:
