@@ -19,12 +19,14 @@ from ..gqa_decode_hf import _scale_ptr
 
 def shared_prefix_pays(batch: int, prefix_len: int) -> bool:
     """Whether reading a prefix once for the batch beats ``paged_flash_decode``
-    over the whole tables, which reads it per sequence.  Measured with 8 KV heads
-    (pools within L2): from 16384 tokens saved on, 16-bit pools gain 10 % (2 x
-    16384 tokens, 29 -> 25 us) to 6.6 x (32 x 16384, 264 -> 40 us), e4m3 pools
-    with groups of 4 lose 15 % at 2 x 16384 and gain 3.9 x at 32 x 16384; below,
-    the two are within a few us of each other."""
-    return batch >= 2 and (batch - 1) * prefix_len >= 16384
+    over the whole tables, which reads it per sequence.  Device times with 8 KV
+    heads, head dim 128, tails of 64, pools within L2, whole tables against shared
+    prefix: 16-bit pools, 32 query heads, 2 x 8192 tokens 21.4 / 18.6 us, 16 x
+    1024 26.3 / 16.4, 32 x 16384 266 / 40; e4m3 pools 2 x 8192 21.2 / 21.2, 16 x
+    1024 22.5 / 17.4, 32 x 16384 168 / 41 (2 x 16384 loses: 26.6 / 28.6).  With
+    4096 tokens saved it still gains (8 x 512 15.3 / 13.4), less than its call
+    costs more on the host."""
+    return batch >= 2 and (batch - 1) * prefix_len >= 8192
 
 
 def paged_flash_decode_shared_prefix(q, k_pool, v_pool, prefix_table, prefix_len, block_table, seq_lens, page_size, *,
