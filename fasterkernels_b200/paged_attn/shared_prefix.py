@@ -22,9 +22,9 @@ def shared_prefix_pays(batch: int, prefix_len: int) -> bool:
     over the whole tables, which reads it per sequence.  Device times with 8 KV
     heads, head dim 128, tails of 64, pools within L2, whole tables against shared
     prefix: 16-bit pools, 32 query heads, 2 x 2048 tokens 14.8 / 14.0 us, 2 x 4096
-    17.2 / 16.0, 16 x 1024 26.3 / 16.4, 32 x 16384 266 / 40; e4m3 pools 2 x 4096
-    18.8 / 17.0, 16 x 1024 22.5 / 17.4, 32 x 16384 168 / 41 (2 x 16384 loses: 26.6
-    / 28.6); head dim 64, 2 x 4096 14.4 / 14.9, 8 x 1024 15.4 / 13.4.  A call takes
+    17.2 / 16.0, 16 x 2048 26.3 / 16.4, 32 x 16384 266 / 40; e4m3 pools 2 x 4096
+    18.8 / 17.0, 16 x 2048 22.5 / 17.4, 32 x 16384 168 / 41 (2 x 16384 loses: 26.6
+    / 28.6); head dim 64, 2 x 4096 14.4 / 14.9, 8 x 2048 15.4 / 13.4.  A call takes
     19 us on the host, one of ``paged_flash_decode`` 24."""
     return batch >= 2 and (batch - 1) * prefix_len >= 4096
 
