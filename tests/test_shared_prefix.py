@@ -118,6 +118,16 @@ def test_long_prefix_crosses_many_segments(dev):
 
 
 @gpu
+@pytest.mark.parametrize("B,tail,P", [(16, 0, 4096), (16, 20, 4096), (16, 80, 8192), (16, 300, 4096), (37, 77, 5003), (64, 200, 2048)])
+def test_prefix_beside_own_parts_of_any_size(dev, B, tail, P):
+    """None, some and all SMs busy with the own part: the prefix is cut differently."""
+    c = make(dev, P, [max(tail - b % 7, 0) for b in range(B)], 16, 4, seed=B + tail)
+    out = call(c)
+    check(c, out)
+    assert torch.equal(out, call(c)) and fk.read_status() == 0
+
+
+@gpu
 @pytest.mark.parametrize("dtype,pool", [(torch.float16, None), (torch.bfloat16, None), (torch.float16, E4M3)])
 def test_sharp_softmax_and_rising_maxima(dev, dtype, pool):
     c = make(dev, 900, [50, 3], 8, 2, dtype=dtype, pool=pool, sinks=True, seed=5, q_scale=6.0)
