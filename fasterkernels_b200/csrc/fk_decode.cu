@@ -612,6 +612,7 @@ int own_part_launch(OwnPart& own, int2* info, int* status, size_t ws_bytes, cuda
   r->hp = hp;
   r->qc = p.qc;
   r->slots = hp == 4 ? 4 * GPAD : GMAX;
+  r->ctas = p.num_ctas;
   r->per_seq = p.qc == 1 ? p.kv_heads / hp : hp == 2 ? p.kv_heads * ((p.qc + 1) / 2) : p.kv_heads * p.qc;
   return FK_OK;
 }

@@ -866,7 +866,7 @@ __global__ void __launch_bounds__(JTHREADS) join_kernel(const __grid_constant__ 
   int item, slot;
   p.own.find(h, grow % p.G, &item, &slot);
   const long long oitem = static_cast<long long>(b) * p.own.per_seq + item;
-  const int2 own = __ldcg(p.own.info + oitem);  // needed last: the prefix's records are read meanwhile
+  const int2 own = p.own.of(oitem);  // needed last: the prefix's records are read meanwhile
   bool past;
   const int plen = prefix_len(p.plen_dev, p.plen, p.blocks, &past);
   const PrefixPlan pl(plen, p.rows, p.kv_heads);

@@ -22,6 +22,14 @@ struct OwnRecords {
   const float* acc;
   const int2* info;
   int hp, qc, slots, per_seq;  // KV heads of an item, query chunks of a KV head, slots, items of a sequence
+  int ctas;                    // of the own part's grid: an item has at most one record in each
+  // The records of item i.  Where a wait of the own part ran out, info[i] may
+  // never have been written: it is then what the scratch held, and taken only if
+  // it names records that exist.
+  __device__ int2 of(long long i) const {
+    const int2 r = __ldcg(info + i);
+    return r.x >= 0 && r.y >= 0 && r.x <= ctas - r.y ? r : make_int2(0, 0);
+  }
   // Item (within its sequence) and slot of query head g of KV head h's group.
   __device__ void find(int h, int g, int* item, int* slot) const {
     if (qc == 1) {

@@ -260,8 +260,9 @@ int fk_qk_norm_rope(const fk_rope_args* args, void* stream);
  *
  * The workspace (fk_shared_prefix_workspace_bytes, 256-byte aligned) is pure
  * scratch: it needs no initial value and carries nothing from call to call, so
- * calls that may overlap only need buffers of their own.  Three kernels are
- * queued on `stream`.
+ * calls that may overlap only need buffers of their own (after
+ * FK_STATUS_TIMEOUT the call's output means nothing, whatever it held).  Three
+ * kernels are queued on `stream`.
  */
 typedef struct fk_prefix_args {
   const void* q;              /* [batch, q_heads, D] */

@@ -401,6 +401,47 @@ def test_bounded_wait_runs_out_and_the_next_call_is_right(dev):
     assert torch.equal(call(c), want) and fk.read_status() == 0
 
 
+def entry_args(c, out, status):
+    """fk_prefix_args of a 16-bit case."""
+    kv = N.dtype_code(c["k"].dtype)
+    B, QH, D = c["q"].shape
+    a = dict(q=c["q"].data_ptr(), k_pool=c["k"].data_ptr(), v_pool=c["v"].data_ptr(), prefix_table=c["table"].data_ptr(),
+             prefix_len_dev=c["plen"].data_ptr(), block_table=c["bt"].data_ptr(), seq_lens=c["seq"].data_ptr(), s_aux=0,
+             out=out.data_ptr(), status=status.data_ptr(), prefix_len=0, prefix_blocks=c["table"].numel(), batch=B, q_heads=QH,
+             kv_heads=c["KVH"], head_dim=D, num_pages=c["k"].shape[0], max_blocks=c["bt"].shape[1], q_dtype=kv, kv_dtype=kv,
+             out_dtype=kv, bt_b=c["bt"].stride(0))
+    for t, names in ((c["q"], "q_b q_h"), (c["k"], "kp_p kp_h kp_s"), (c["v"], "vp_p vp_h vp_s"), (out, "o_b o_h")):
+        a.update(zip(names.split(), t.stride()))
+    return _args(**a)
+
+
+@gpu
+@pytest.mark.parametrize("word", [0x3f800000, 0x7fffffff, -1, 1])
+@pytest.mark.parametrize("lens", [[20, 33], [4000, 0, 7]])
+def test_a_wait_that_ran_out_over_any_scratch_is_a_status(dev, word, lens):
+    """The own part gives up before it says where its records are: what the
+    scratch held there must not be taken for them."""
+    c = make(dev, 1500, lens, 16, 2, seed=10)
+    want = call(c)
+    lib = N.lib()
+    need = lib.fk_shared_prefix_workspace_bytes(0, len(lens), 16, 2, 128, N.FK_DTYPE_F16)
+    ws = torch.full((need // 4,), word, dtype=torch.int32, device=dev)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    out = torch.empty_like(want)
+    stream = N.stream_of(dev)
+    assert lib.fk_debug_configure(100_000_000, 1) == 0
+    try:
+        assert lib.fk_paged_shared_prefix_decode(entry_args(c, out, status), ws.data_ptr(), need, stream) == 0
+        torch.cuda.synchronize()
+    finally:
+        assert lib.fk_debug_configure(4_000_000_000, 0) == 0
+    assert int(status) == N.FK_STATUS_TIMEOUT
+    status.zero_()
+    assert lib.fk_paged_shared_prefix_decode(entry_args(c, out, status), ws.data_ptr(), need, stream) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and int(status) == 0
+
+
 @gpu
 def test_wrapper_refusals(dev):
     c = make(dev, 100, [20, 7], 8, 2, seed=1)
