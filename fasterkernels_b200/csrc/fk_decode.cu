@@ -599,9 +599,12 @@ int own_part_prepare(OwnPart* own, const fk_prefix_args& a, void* workspace, int
   return FK_OK;
 }
 
-int own_part_launch(OwnPart& own, int2* info, int* status, size_t ws_bytes, cudaStream_t stream, OwnRecords* r) {
+int own_part_launch(OwnPart& own, int2* info, unsigned long long* ticket, unsigned long long ticket_value, int* status,
+                    size_t ws_bytes, cudaStream_t stream, OwnRecords* r) {
   Params& p = own.p;
   p.part_info = info;
+  p.part_ticket = ticket;
+  p.part_ticket_value = g_inject.load() == 4 ? 0 : ticket_value;
   if (status != nullptr) p.status = status;  // else the workspace's first word, which nobody reads
   const int rc = launch<PAGED>(p, own.kv, own.device, ws_bytes, stream);
   if (rc != FK_OK) return rc;
@@ -686,7 +689,7 @@ extern "C" int fk_profile_end(float* kernel_ms, int* launches) {
 extern "C" int fk_debug_configure(unsigned long long wait_ns, int inject) {
   if (wait_ns < 1000000ull || wait_ns > 60000000000ull)
     return fail(FK_ERR_INVALID_ARG, "wait_ns must be in [1 ms, 60 s]");
-  if (inject != 0 && inject != 1) return fail(FK_ERR_INVALID_ARG, "inject must be 0 or 1");
+  if (inject != 0 && inject != 1 && inject != 4) return fail(FK_ERR_INVALID_ARG, "inject must be 0, 1 or 4");
   g_wait_ns.store(wait_ns);
   g_inject.store(inject);
   return FK_OK;

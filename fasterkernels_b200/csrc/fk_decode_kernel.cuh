@@ -203,6 +203,8 @@ struct Params {
   // too, stays in the workspace for the join, item i's being records i + x .. i +
   // x + y - 1 of part_info[i] = (x, y); nothing is merged or written to `out`.
   int2* part_info;
+  unsigned long long* part_ticket;  // set to part_ticket_value after this grid's wait for what precedes it
+  unsigned long long part_ticket_value;
   int* status;         // FK_STATUS_* word: the workspace's first, or the caller's
   unsigned long long wait_ns;  // bound of every mbarrier wait
   int inject;                  // test hook: 1 = each CTA's producer withholds its first stage
@@ -471,6 +473,8 @@ __global__ void __launch_bounds__(THREADS, KvCfg<KV, D, CP>::MINB) decode_split_
   // which returns once the prerequisite grid has completed and its writes are
   // visible.
   grid_dependency_wait();
+  if (LAYOUT == PAGED && p.part_info != nullptr && blockIdx.x == 0 && threadIdx.x == 0)
+    st_release_gpu(p.part_ticket, p.part_ticket_value);
   // Plan, with every thread of the CTA: thread t sums the granules of
   // sequences [t*bpt, (t+1)*bpt) (independent loads, one round trip); each
   // warp scans its 32 sums in parallel, and every thread adds the totals of

@@ -42,8 +42,9 @@ struct OwnRecords {
     }
   }
 };
-// Nothing in its workspace need be set before.
-int own_part_launch(OwnPart& own, int2* info, int* status, size_t ws_bytes, cudaStream_t stream, OwnRecords* records);
+// Nothing in its workspace need be set before.  *ticket is ticket_value from
+// when the kernel has waited for what precedes it in the stream.
+int own_part_launch(OwnPart& own, int2* info, unsigned long long* ticket, unsigned long long ticket_value, int* status, size_t ws_bytes, cudaStream_t stream, OwnRecords* records);
 // A tensor map with 128-byte swizzle (fk_decode.cu).
 int encode_map(CUtensorMap* map, int kv, int rank, const void* base, const uint64_t* dims, const uint64_t* strides_b,
                const uint32_t* box);

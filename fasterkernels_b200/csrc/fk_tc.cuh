@@ -129,6 +129,9 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
 // Make this thread's writes to shared memory visible to the tensor cores.
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// Let this thread's asynchronous copies read global memory that it may read itself.
+__device__ __forceinline__ void fence_async_global() { asm volatile("fence.proxy.async.global;" ::: "memory"); }
+
 // 16-byte asynchronous copy, zeros when !ok.
 __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool ok) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");

@@ -348,7 +348,9 @@ int fk_decode_num_ctas(int device, int kv_dtype, int kv_heads);
  * nothing for its first pipeline stage, so its consumers' wait runs out, the
  * kernel sets FK_STATUS_TIMEOUT and returns (no fault; before exiting, each
  * CTA waits, bounded, for the copies it issued to land).  Clear the workspace after a timeout: arrival counters of split
- * items may be left mid-count.  inject = 0 restores normal operation.
+ * items may be left mid-count.  inject = 4 makes the own part of a shared-prefix
+ * decode withhold its ticket, so that the prefix kernel waits for it (results
+ * are the same).  inject = 0 restores normal operation.
  */
 int fk_debug_configure(unsigned long long wait_ns, int inject);
 

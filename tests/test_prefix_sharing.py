@@ -239,6 +239,66 @@ def test_inputs_written_right_before_the_call(dev, graphed):
     assert fk.read_status() == 0
 
 
+@gpu
+@pytest.mark.parametrize("inject", [0, 4])
+@pytest.mark.parametrize("graphed", [False, True])
+def test_inputs_written_right_before_the_call_against_64_bits(dev, graphed, inject):
+    """Every input of a step is written by the kernels right before it: q, a page
+    of the prefix, the own tokens, both tables, both lengths.  Against attention
+    over what was written, with the prefix kernel taking the own part's word for
+    it (inject 0) and waiting for it (4)."""
+    from fasterkernels_b200 import _native as N
+    B, QH, KVH, D, blocks = 3, 4, 2, 128, 20
+    g = torch.Generator(device=dev).manual_seed(19)
+    pages = blocks + 2 * B
+    kp, vp = (torch.randn(pages, KVH, 16, D, generator=g, device=dev).half() for _ in range(2))
+    src_k, src_v = kp.clone(), vp.clone()
+    perm = torch.randperm(pages, generator=g, device=dev).to(torch.int32)
+    table, bt = perm[:blocks].clone(), perm[blocks:].view(B, 2).clone()
+    src_table, src_bt = table.clone(), bt.clone()
+    q, src_q = (torch.randn(B, QH, D, generator=g, device=dev).half() for _ in range(2))
+    lens, src_lens = (torch.zeros(B, dtype=torch.int32, device=dev) for _ in range(2))
+    plen, src_plen = (torch.full((1,), 16 * blocks, dtype=torch.int32, device=dev) for _ in range(2))
+
+    def step():
+        for dst, src in ((kp, src_k), (vp, src_v), (table, src_table), (bt, src_bt), (lens, src_lens), (plen, src_plen), (q, src_q)):
+            dst.copy_(src)
+        return fk.paged_flash_decode_shared_prefix(q, kp, vp, table, plen, bt, lens, 16)
+
+    lib = N.lib()
+    assert lib.fk_debug_configure(4_000_000_000, inject) == 0
+    try:
+        out = step()
+        if graphed:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                out = step()
+        for i in range(40):
+            src_q.normal_(generator=g)
+            src_k.normal_(generator=g)
+            src_v.normal_(generator=g)
+            perm = torch.randperm(pages, generator=g, device=dev).to(torch.int32)
+            src_table.copy_(perm[:blocks])
+            src_bt.copy_(perm[blocks:].view(B, 2))
+            own, prefix = [(5 * i + 11 * b) % 33 for b in range(B)], 1 + (37 * i) % (16 * blocks)
+            src_lens.copy_(torch.tensor(own))
+            src_plen.fill_(prefix)
+            torch.cuda.synchronize()
+            if graphed:
+                graph.replay()
+            else:
+                out = step()
+            pk, pv = (x[src_table.long()].transpose(0, 1).reshape(KVH, -1, D) for x in (src_k, src_v))
+            tk, tv = (x[src_bt.long()].transpose(1, 2).reshape(B, KVH, -1, D) for x in (src_k, src_v))
+            args = (src_q.double(), pk, pv, prefix, tk, tv, own)
+            ref = shared_prefix_ref(*args)
+            bound = attention_bound(*args, None, ref, torch.float16, out.dtype)
+            assert bool(((out.double() - ref).abs() <= bound).all()), i
+    finally:
+        assert lib.fk_debug_configure(4_000_000_000, 0) == 0
+    assert fk.read_status() == 0
+
+
 class _Module:
     is_causal = True
 
