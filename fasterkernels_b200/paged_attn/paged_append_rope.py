@@ -66,8 +66,8 @@ def paged_kv_append_rope(q, k, v, k_pool, v_pool, block_table, positions, cos, s
     if positions.numel() != T:
         raise ValueError("positions must have one entry per token")
     _check_table(cos, sin, D, dev)
-    _check_weight(q_weight, "q_weight", D, dev)
-    _check_weight(k_weight, "k_weight", D, dev)
+    q_weight = _check_weight(q_weight, "q_weight", D, dev)
+    k_weight = _check_weight(k_weight, "k_weight", D, dev)
     sk = sv = None
     if pool_code == N.FK_DTYPE_E4M3:
         if scale_k is None or scale_v is None:

@@ -83,8 +83,12 @@ def _check_table(cos, sin, D, dev):
 
 
 def _check_weight(w, name, D, dev):
-    if w is not None and (w.device != dev or w.numel() != D or w.dtype not in _TABLE):
+    """w as the kernel reads it, its D entries one after another."""
+    if w is None:
+        return None
+    if w.device != dev or w.numel() != D or w.dtype not in _TABLE:
         raise ValueError(f"{name} must have head_dim entries (float32, float16 or bfloat16) on q's device")
+    return w if w.is_contiguous() else w.contiguous()
 
 
 def _check_out(out, like, name):
@@ -125,8 +129,8 @@ def qk_norm_rope(q, k, cos, sin, positions=None, *, q_weight=None, k_weight=None
             raise ValueError("positions must have one entry per token")
     elif R == 0:
         positions = torch.zeros(T, dtype=torch.int32, device=dev)
-    _check_weight(q_weight, "q_weight", D, dev)
-    _check_weight(k_weight, "k_weight", D, dev)
+    q_weight = _check_weight(q_weight, "q_weight", D, dev)
+    k_weight = _check_weight(k_weight, "k_weight", D, dev)
     q_out = _check_out(q_out, q, "q_out")
     k_out = _check_out(k_out, k, "k_out")
     _check_status(status, dev)

@@ -157,6 +157,46 @@ def test_norm_rope_types_of_tables_and_weights_and_one_weight_only(dev):
     _inside(ko, *norm_rope_ref(k, cos, sin, row))
 
 
+def _scattered_weights(D, dtype, device):
+    """Norm weights whose entries do not lie one after another."""
+    g = torch.Generator().manual_seed(23)
+    layers = (1 + 0.2 * torch.randn(D, 8, generator=g)).to(dtype).to(device)
+    return [layers[:, 3], layers.reshape(-1)[::8], layers[:, 2:3], layers[3:4, :1].expand(D, 1), layers[0, :1].expand(D),
+            layers.t()[5:6]]
+
+
+def test_weights_are_handed_on_contiguous():
+    from fasterkernels_b200.qk_norm_rope import _check_weight
+    for w in _scattered_weights(64, torch.float16, "cpu"):
+        got = _check_weight(w, "q_weight", 64, w.device)
+        assert got.is_contiguous() and torch.equal(got.reshape(-1), w.reshape(-1))
+    w = torch.ones(64)
+    assert _check_weight(w, "q_weight", 64, w.device) is w and _check_weight(None, "q_weight", 64, w.device) is None
+
+
+@gpu
+@pytest.mark.parametrize("T", [5, 4000])
+def test_norm_weights_of_any_layout(dev, T):
+    """A column of stacked parameters, every eighth entry, an expanded one."""
+    D = 128
+    q, k, v = _heads(dev, T, 4, 2, D, torch.float16, seed=7)
+    cos, sin = fk.rope_table(64, D, device=dev)
+    pos = torch.arange(T, device=dev, dtype=torch.int32) % 64
+    kp, vp = (torch.zeros(T // 16 + 1, 2, 16, D, dtype=torch.float16, device=dev) for _ in range(2))
+    bt = torch.arange(T // 16 + 1, dtype=torch.int32, device=dev)[None]
+    zero = torch.zeros(T, dtype=torch.int32, device=dev)
+    at = torch.arange(T, dtype=torch.int32, device=dev)
+    for dtype in (torch.float32, torch.float16):
+        for w in _scattered_weights(D, dtype, dev):
+            qo, ko = fk.qk_norm_rope(q, k, cos, sin, pos, q_weight=w, k_weight=w)
+            for got, x in ((qo, q), (ko, k)):
+                _inside(got, *norm_rope_ref(x, cos, sin, pos, w.reshape(-1)))
+            qa = fk.paged_kv_append_rope(q, k, v, kp, vp, bt, at, None, None, seq_ids=zero, q_weight=w, k_weight=w)
+            _inside(qa, *norm_rope_ref(q, None, None, at, w.reshape(-1)))
+            kept = kp.transpose(1, 2).reshape(-1, 2, D)[:T]
+            _inside(kept, *norm_rope_ref(k, None, None, at, w.reshape(-1)))
+
+
 @gpu
 def test_norm_rope_small_and_large_rows(dev):
     # rows of zeros stay zero (eps keeps the norm finite); rows near the type's ends stay inside the bound
