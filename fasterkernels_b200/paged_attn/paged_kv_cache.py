@@ -163,12 +163,15 @@ class PagedKVCache:
         prompt token by token, benchmarks/run_hf_triton_fp8_paged.py:113-117).
         Pages are allocated on the host for max(T, reserve) tokens, so a
         caller can fix the block table for the decode steps that follow.
-        The sequence length becomes T (the same T for every layer)."""
+        The sequence length becomes T (the same T for every layer).  A sequence
+        that shares pages (``fork_sequence``) is refused."""
         if k.dim() != 3 or k.shape != v.shape or k.shape[0] != self.num_kv_heads or k.shape[2] != self.head_dim:
             raise ValueError("k / v must be [num_kv_heads, T, head_dim]")
         T = int(k.shape[1])
         pages = self._pages[seq_id]
-        if any(p in self._page_refs for p in pages[: (T + PAGE_SIZE - 1) // PAGE_SIZE]):
+        # An empty prompt too: the tokens after it would go to the first page.
+        # Who holds a page holds those before it, so the first one tells.
+        if pages and pages[0] in self._page_refs:
             raise RuntimeError("write_prefill would overwrite pages shared with another sequence")
         need = (max(T, int(reserve)) + PAGE_SIZE - 1) // PAGE_SIZE
         if need > self.max_blocks_per_seq:

@@ -76,6 +76,24 @@ def test_fork_refusals():
         prefill(c, 1, 5)
 
 
+def test_an_empty_prefill_of_a_sequence_with_shared_pages_is_refused():
+    c = make(layers=1)
+    a = c.allocate_sequence()
+    prefill(c, a, 40)
+    b = c.fork_sequence(a, 32)
+    before = c.k_pool.clone()
+    for sid in (a, b):
+        with pytest.raises(RuntimeError, match="shared"):
+            c.write_prefill(sid, 0, c.k_pool.new_zeros(2, 0, 128), c.k_pool.new_zeros(2, 0, 128))
+    assert (c.seq_len(a), c.seq_len(b), c.shared_prefix_pages([a, b])) == (40, 32, 2)
+    c.append_kv(b, 0, torch.ones(1, 2, 1, 128), torch.ones(1, 2, 1, 128))
+    pages = c.block_table[a, :3].long()
+    assert torch.equal(c.k_pool[0, pages], before[0, pages])
+    c.free_sequence(b)  # a holds its pages alone again
+    c.write_prefill(a, 0, c.k_pool.new_zeros(2, 0, 128), c.k_pool.new_zeros(2, 0, 128))
+    assert c.seq_len(a) == 0
+
+
 def test_shared_prefix_of_unrelated_single_and_repeated_sequences():
     c = make()
     a, b = c.allocate_sequence(), c.allocate_sequence()
