@@ -139,23 +139,60 @@ def qk_norm_rope(q, k, cos, sin, positions=None, *, q_weight=None, k_weight=None
     return q_out, k_out
 
 
-def custom_hf_apply_rotary_pos_emb(q, k, cos, sin, unsqueeze_dim: int = 1, **kwargs):
+def _angles_once(t, tables):
+    """Each angle of an HF table [.., columns] once: [.., R / 2]."""
+    return t[..., : t.shape[-1] // 2] if tables == "halves" else t[..., ::2].contiguous() if tables == "pairs" else t
+
+
+def _hf_tables(cos, D, tables, interleaved):
+    """How the tables of an HF model hold their angles, where ``tables`` and the
+    number of columns say it; refused where they do not."""
+    cols = cos.shape[-1]
+    if tables not in (None, "halves", "pairs", "once"):
+        raise ValueError("tables must be 'halves', 'pairs' or 'once'")
+    if tables is None:
+        if interleaved:
+            raise ValueError("interleaved pairs come with tables='pairs' (each angle twice, side by side) or 'halves'")
+        if 2 * cols == D:
+            raise ValueError("cos / sin of head_dim / 2 columns are all angles once (tables='once') or a rotation of half "
+                             "the dims (tables='halves'): pass tables")
+        tables = "halves"
+    R = 2 * cols if tables == "once" else cols
+    if R == 0 or R > D or R % 16:
+        raise ValueError(f"cos / sin of {cols} columns rotate {R} of {D} dims: must be a multiple of 16 up to the head dim")
+    return tables
+
+
+def custom_hf_apply_rotary_pos_emb(q, k, cos, sin, unsqueeze_dim: int = 1, *, tables=None, interleaved: bool = False,
+                                   **kwargs):
     """Drop-in for the ``apply_rotary_pos_emb`` of transformers' model files, the
     way ``custom_hf_decode_attention_forward`` stands in for their attention:
     q [B, Q_H, S, D], k [B, KV_H, S, D] (``unsqueeze_dim=2``: heads after S),
-    cos / sin [B or 1, S, R] with the half-split angles repeated.  Both are
-    rotated by one kernel; returned in the layout they came in."""
+    cos / sin [B or 1, S, columns].  Both are rotated by one kernel; returned in
+    the layout they came in.
+
+    As it is, it stands in for the function of Llama, Qwen, Mistral and most
+    others: half-split pairs, the angles repeated in the second half of the
+    columns, one column per rotated dim.  Model files that pair or hold them
+    otherwise have the same signature, so these two say which, bound with
+    ``functools.partial``: ``interleaved`` rotates dims (2 i, 2 i + 1);
+    ``tables`` says how the columns hold the angles, "halves" (a, b, a, b), "pairs"
+    (a, a, b, b) or "once" (a, b).  GPT-OSS: tables="once".  Cohere:
+    interleaved=True, tables="pairs".  Ernie 4.5, GLM, Helium: interleaved=True,
+    tables="halves".  GLM-4 MoE (half of the dims rotated): tables="halves".
+    Tables of head_dim / 2 columns are refused without ``tables``."""
     if q.dim() != 4 or k.dim() != 4 or cos.dim() != 3 or unsqueeze_dim not in (1, 2):
         raise ValueError("q, k must be 4-D, cos / sin [B, S, R], unsqueeze_dim 1 or 2")
     if unsqueeze_dim == 1:
         q, k = q.transpose(1, 2), k.transpose(1, 2)
     B, S = q.shape[:2]
-    if cos.shape[1] != S or cos.shape[0] not in (1, B):
+    if cos.shape[1] != S or cos.shape[0] not in (1, B) or sin.shape != cos.shape:
         raise ValueError("cos / sin must have q's sequence length and its batch (or 1)")
-    half = cos.shape[2] // 2
-    cos, sin = (t.reshape(-1, 2 * half)[:, :half] for t in (cos, sin))
+    tables = _hf_tables(cos, q.shape[-1], tables, interleaved)
+    cos, sin = (_angles_once(t.reshape(-1, t.shape[-1]), tables) for t in (cos, sin))
     if cos.dtype not in _TABLE:
         cos, sin = cos.float(), sin.float()
-    qo, ko = qk_norm_rope(q.reshape(B * S, *q.shape[2:]), k.reshape(B * S, *k.shape[2:]), cos, sin)
+    qo, ko = qk_norm_rope(q.reshape(B * S, *q.shape[2:]), k.reshape(B * S, *k.shape[2:]), cos, sin,
+                          interleaved=interleaved)
     qo, ko = qo.view(q.shape), ko.view(k.shape)
     return (qo.transpose(1, 2), ko.transpose(1, 2)) if unsqueeze_dim == 1 else (qo, ko)

@@ -629,6 +629,73 @@ def test_hf_rotary_drop_in_inside_a_random_weight_model(dev, monkeypatch):
     torch.testing.assert_close(got, want, atol=3e-2, rtol=3e-2)
 
 
+# model file -> what the drop-in takes for it, rotated dims of 128, columns
+_HF_LAYOUTS = {
+    "llama": (dict(), 128, 128),
+    "phi3": (dict(), 96, 96),
+    "glm4_moe": (dict(tables="halves"), 64, 64),
+    "gpt_oss": (dict(tables="once"), 128, 64),
+    "cohere": (dict(tables="pairs", interleaved=True), 128, 128),
+    "ernie4_5": (dict(tables="halves", interleaved=True), 128, 128),
+    "glm": (dict(tables="halves", interleaved=True), 64, 64),
+}
+
+
+def _hf_case(model, device, dtype):
+    import importlib
+    kw, R, cols = _HF_LAYOUTS[model]
+    own = importlib.import_module(f"transformers.models.{model}.modeling_{model}").apply_rotary_pos_emb
+    g = torch.Generator().manual_seed(31)
+    B, S, D = 2, 9, 128
+    q, k = (torch.randn(B, h, S, D, generator=g).to(dtype).to(device) for h in (4, 2))
+    ang = 6 * torch.rand(B, S, R // 2, generator=g)
+    c, s = ang.cos().to(device), ang.sin().to(device)
+    wide = [t if cols == R // 2 else t.repeat_interleave(2, -1) if kw.get("tables") == "pairs" else torch.cat([t, t], -1)
+            for t in (c, s)]
+    assert wide[0].shape[-1] == cols
+    return kw, own, q, k, *wide, c.reshape(B * S, -1), s.reshape(B * S, -1)
+
+
+@pytest.mark.parametrize("model", _HF_LAYOUTS)
+def test_hf_table_layouts_are_those_of_the_model_files(model):
+    from fasterkernels_b200.qk_norm_rope import _angles_once, _hf_tables
+    kw, own, q, k, cos, sin, *once = _hf_case(model, "cpu", torch.float32)
+    tables = _hf_tables(cos, 128, kw.get("tables"), kw.get("interleaved", False))
+    c, s = (_angles_once(t.reshape(-1, t.shape[-1]), tables) for t in (cos, sin))
+    assert torch.equal(c, once[0]) and torch.equal(s, once[1])
+    row = torch.arange(18)
+    for want, x in zip(own(q, k, cos, sin), (q, k)):
+        ref, amp = norm_rope_ref(x.transpose(1, 2).reshape(18, -1, 128), c, s, row, interleaved=kw.get("interleaved", False))
+        # f32 there: two products and a sum, half a step each
+        assert bool(((want.transpose(1, 2).reshape(ref.shape).double() - ref).abs() <= 3 * 2.0 ** -24 * amp).all())
+
+
+def test_hf_tables_that_do_not_say_what_they_are_are_refused():
+    q, k = torch.zeros(1, 4, 3, 128), torch.zeros(1, 2, 3, 128)
+    t = lambda cols: torch.zeros(1, 3, cols)  # noqa: E731
+    f = fk.custom_hf_apply_rotary_pos_emb
+    for cols, kw, match in ((64, {}, "tables"), (128, dict(interleaved=True), "tables"), (128, dict(tables="twice"), "tables must"),
+                            (128, dict(tables="once"), "256 of 128"), (33, {}, "33 columns"), (256, {}, "256 columns"),
+                            (0, {}, "0 columns"), (8, dict(tables="pairs"), "multiple of 16")):
+        with pytest.raises(ValueError, match=match):
+            f(q, k, t(cols), t(cols), **kw)
+    with pytest.raises(ValueError, match="sequence length"):
+        f(q, k, t(128), t(64))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("model", _HF_LAYOUTS)
+def test_hf_rotary_drop_in_for_each_table_layout(dev, model, dtype):
+    kw, own, q, k, cos, sin, c, s = _hf_case(model, dev, dtype)
+    got = fk.custom_hf_apply_rotary_pos_emb(q, k, cos, sin, **kw)
+    row = torch.arange(18, device=dev)
+    for g, want, x in zip(got, own(q.float(), k.float(), cos, sin), (q, k)):
+        ref, amp = norm_rope_ref(x.transpose(1, 2).reshape(18, -1, 128), c, s, row, interleaved=kw.get("interleaved", False))
+        _inside(g.transpose(1, 2).reshape(ref.shape), ref, amp)
+        assert bool(((want.transpose(1, 2).reshape(ref.shape).double() - ref).abs() <= 2.0 ** -20 * amp).all())
+
+
 def test_custom_ops_declare_what_they_write():
     ns = torch.ops.fasterkernels_b200
     for name, mutated in (("qk_norm_rope", {"q_out", "k_out", "k_pool", "v_pool", "status"}),
