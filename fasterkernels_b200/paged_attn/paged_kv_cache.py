@@ -24,6 +24,8 @@ from typing import Dict, List
 
 import torch
 
+from .. import _native as N
+
 PAGE_SIZE = 16
 
 
@@ -42,6 +44,8 @@ class PagedKVCache:
         shape = (self.num_layers, self.num_pages, self.num_kv_heads, PAGE_SIZE, self.head_dim)
         self.k_pool = torch.zeros(shape, dtype=self.dtype, device=self.device)
         self.v_pool = torch.zeros_like(self.k_pool)
+        if self.k_pool.is_cuda:
+            N.status_word(self.k_pool.device)  # made here: a captured step may be the first to name it
         self.block_table = torch.full((self.max_seqs, self.max_blocks_per_seq), -1, dtype=torch.int32,
                                       device=self.device)
         self._seq_lens: List[int] = [0] * self.max_seqs
@@ -57,6 +61,7 @@ class PagedKVCache:
         self._step_bt = None
         self._step_pos = None
         self._step_seq = None  # block-table row of each token (None: token t is row t)
+        self._step_last = -1   # the step's largest position
         self._page_refs: Dict[int, int] = {}  # holders of the pages that have more than one
         self._shared_runs: Dict[tuple, int] = {}  # shared_prefix_pages by sequences, until the next fork or free
 
@@ -225,6 +230,7 @@ class PagedKVCache:
         self._step_ids = list(seq_ids)
         self._step_counts = [1] * len(seq_ids)
         self._step_seq = None
+        self._step_last = max((self._seq_lens[s] for s in seq_ids), default=-1)
         self._step_bt = self.get_block_table_tensor(self._step_ids)
         self._step_pos = self.get_seq_lens_tensor(self._step_ids)
         return self._step_bt, self._step_pos, self._step_pos + 1
@@ -261,25 +267,32 @@ class PagedKVCache:
             upd = torch.tensor([rows, cols, vals], dtype=torch.int64).to(self.device, non_blocking=True)
             self.block_table[upd[0], upd[1]] = upd[2].to(torch.int32)
         self._step_ids, self._step_counts = list(seq_ids), counts
+        self._step_last = max((self._seq_lens[s] + c - 1 for s, c in zip(seq_ids, counts) if c), default=-1)
         self._step_bt = self.get_block_table_tensor(self._step_ids)
         place = torch.tensor([pos, seq], dtype=torch.int32).to(self.device, non_blocking=True)
         self._step_pos, self._step_seq = place[0], place[1]
         return self._step_bt, self._step_pos, self._step_seq
 
     def append_qkv_batch(self, layer_idx: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos, sin, *, q_weight=None,
-                         k_weight=None, eps: float = 1e-6, interleaved: bool = False, q_out=None, k_out=None):
+                         k_weight=None, eps: float = 1e-6, interleaved: bool = False, q_out=None, k_out=None, status=None):
         """Norm and rotate this step's q and k and write k and v into layer
         ``layer_idx`` with one kernel: q [T, Q_H, D], k / v [T, KV_H, D] of the
         tokens of ``begin_step`` (T = B) or ``begin_chunk``; the other arguments
-        are those of ``paged_kv_append_rope``.  Returns the rotated q."""
+        are those of ``paged_kv_append_rope``.  A step that goes past the rows of
+        cos / sin is refused; what the kernel finds is in ``read_status()``, or in
+        ``status``.  Returns the rotated q."""
         from .paged_append_rope import paged_kv_append_rope
         if self._step_pos is None:
             raise RuntimeError("call begin_step() or begin_chunk() before append_qkv_batch()")
+        if cos is not None and self._step_last >= cos.shape[0]:
+            raise ValueError(f"position {self._step_last} of this step is past the {cos.shape[0]} rows of cos / sin")
+        if status is None and self.k_pool.is_cuda:
+            status = N.status_word(self.k_pool.device)
         e4m3 = self.dtype == torch.float8_e4m3fn
         return paged_kv_append_rope(q, k, v, self.k_pool[layer_idx], self.v_pool[layer_idx], self._step_bt, self._step_pos,
                                     cos, sin, seq_ids=self._step_seq, q_weight=q_weight, k_weight=k_weight, eps=eps,
                                     interleaved=interleaved, scale_k=self.k_scale if e4m3 else None,
-                                    scale_v=self.v_scale if e4m3 else None, q_out=q_out, k_out=k_out)
+                                    scale_v=self.v_scale if e4m3 else None, q_out=q_out, k_out=k_out, status=status)
 
     def append_kv_batch(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor) -> None:
         """Write this step's K/V ([B, KV_H, 128] or [B, KV_H, 1, 128]) of every

@@ -128,6 +128,30 @@ def test_begin_chunk_places_ragged_tokens_and_commits_their_counts():
         c.append_qkv_batch(0, None, None, None, None, None)
 
 
+@pytest.mark.parametrize("chunk", [False, True])
+def test_a_step_past_the_cos_sin_rows_is_refused_before_anything_is_appended(chunk):
+    c = make(layers=1)
+    a, b = c.allocate_sequence(), c.allocate_sequence()
+    prefill(c, a, 40)
+    prefill(c, b, 7)
+    before = c.k_pool.clone()
+    T = 6 if chunk else 2
+    x = torch.zeros(T, 2, 128, dtype=c.dtype)
+    if chunk:
+        c.begin_chunk([b, a], [4, 2])  # positions 7 .. 10 and 40, 41
+    else:
+        c.begin_step([b, a])           # 7 and 40
+    table = torch.zeros(41 if chunk else 40, 64)
+    with pytest.raises(ValueError, match=f"position {41 if chunk else 40}"):
+        c.append_qkv_batch(0, x, x, x, table, table)
+    assert torch.equal(c.k_pool, before) and (c.seq_len(a), c.seq_len(b)) == (40, 7)
+    with pytest.raises(ValueError, match="CUDA"):  # one more row, or no rotation: on to the kernel's own checks
+        c.append_qkv_batch(0, x, x, x, *(torch.zeros(42, 64) for _ in range(2)))
+    with pytest.raises(ValueError, match="CUDA"):
+        c.append_qkv_batch(0, x, x, x, None, None)
+    c.end_step()
+
+
 # ------------------------------------------------------------------ GPU
 @pytest.fixture(scope="module")
 def dev():
@@ -255,6 +279,52 @@ def test_inputs_written_right_before_the_call(dev, graphed):
         torch.cuda.synchronize()
         assert torch.equal(got, decode()), i
     assert fk.read_status() == 0
+
+
+@gpu
+def test_the_cache_reports_what_a_step_could_not_append(dev):
+    """A step whose positions or pages change behind the cache's back (here by
+    hand, as a replayed graph could) leaves its bit in read_status()."""
+    from fasterkernels_b200 import _native as N
+    c = make(pages=8, device=str(dev), layers=1)
+    a = c.allocate_sequence()
+    x = torch.randn(1, 2, 128, device=dev).half()
+    cos, sin = fk.rope_table(64, 128, device=dev)
+    fk.read_status()
+    for what, bit in ((None, 0), ("pos", N.FK_STATUS_BAD_POSITION), ("bt", N.FK_STATUS_BAD_PAGE)):
+        c.begin_step([a])
+        if what == "pos":
+            c._step_pos.fill_(64)
+        elif what == "bt":
+            c._step_bt.fill_(-1)
+        c.append_qkv_batch(0, x, x, x, cos, sin)
+        c.end_step()
+        assert fk.read_status() == bit
+    mine = torch.zeros(1, dtype=torch.int32, device=dev)
+    c.begin_step([a])
+    c._step_pos.fill_(-1)
+    c.append_qkv_batch(0, x, x, x, cos, sin, status=mine)
+    assert int(mine) == N.FK_STATUS_BAD_POSITION and fk.read_status() == 0
+
+
+@gpu
+def test_the_first_append_of_a_cache_can_be_a_captured_one(dev):
+    from fasterkernels_b200 import _native as N
+    words = dict(N._status)
+    N._status.clear()
+    try:
+        c = make(pages=8, device=str(dev), layers=1)
+        a = c.allocate_sequence()
+        x = torch.randn(1, 2, 128, device=dev).half()
+        cos, sin = fk.rope_table(64, 128, device=dev)
+        c.begin_step([a])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            q = c.append_qkv_batch(0, x, x, x, cos, sin)
+        graph.replay()
+        assert torch.equal(q, x) and torch.equal(c.k_pool[0, c._pages[a][0], :, 0], x[0]) and fk.read_status() == 0
+    finally:
+        N._status.update(words)
 
 
 @gpu
