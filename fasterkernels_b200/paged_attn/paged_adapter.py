@@ -91,7 +91,8 @@ def custom_paged_attention_forward(module, query_states, key_states, value_state
         kw = dict(s_aux=_module_sinks(module, q_heads, query_states.device),
                   scale_k=cache.k_scale if e4m3 else None, scale_v=cache.v_scale if e4m3 else None,
                   out_dtype=query_states.dtype if e4m3 else None)
-        q, kp, vp, n = query_states.squeeze(2), cache.k_pool[layer], cache.v_pool[layer], _BOUND.shared
+        # detached: no decode call has a backward pass, and one of the two refuses
+        q, kp, vp, n = query_states.detach().squeeze(2), cache.k_pool[layer], cache.v_pool[layer], _BOUND.shared
         if n:
             out = paged_flash_decode_shared_prefix(q, kp, vp, _BOUND.bt[0, :n], n * PAGE_SIZE, _BOUND.bt[:, n:], _BOUND.own,
                                                    PAGE_SIZE, **kw)

@@ -396,6 +396,31 @@ class _Module:
 
 
 @gpu
+@pytest.mark.parametrize("forked", [False, True])
+def test_paged_adapter_with_queries_that_require_grad(dev, forked):
+    """A model run without no_grad: the same step as under it, forks or not."""
+    outs = []
+    for grad in (False, True):
+        c = make(pages=2 * 290, seqs=3, blocks=290, device=str(dev), layers=2)
+        g = torch.Generator(device=dev).manual_seed(15)
+        k = torch.randn(2, 2, 2, 4416, 128, generator=g, device=dev).half()
+        a = c.allocate_sequence()
+        for layer in range(2):
+            c.write_prefill(a, layer, k[layer, 0], k[layer, 1])
+        ids = [a, c.fork_sequence(a, 4416)] if forked else [a]
+        q = torch.randn(len(ids), 8, 1, 128, generator=g, device=dev).half().requires_grad_(grad)
+        kv = torch.randn(2, len(ids), 2, 1, 128, generator=g, device=dev).half().requires_grad_(grad)
+        fk.set_paged_attention_cache(c, ids)
+        try:
+            outs.append([fk.custom_paged_attention_forward(_Module(i), q, kv[0], kv[1], None, 128 ** -0.5)[0] for i in range(2)])
+        finally:
+            fk.set_paged_attention_cache(None, [])
+        assert [c.seq_len(s) for s in ids] == [4417] * len(ids)
+    for x, y in zip(*outs):
+        assert torch.equal(x, y) and not y.requires_grad
+
+
+@gpu
 @pytest.mark.parametrize("pool", [torch.float16, E4M3])
 def test_paged_adapter_decodes_forked_sequences_behind_their_prefix(dev, pool, monkeypatch):
     """Forked sequences through the adapter give what unforked copies of them
