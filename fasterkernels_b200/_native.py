@@ -139,6 +139,13 @@ def raw_stream(index: int) -> int:
 
 
 # ---------------------------------------------------------------- workspace
+def _kept_zeros(size: int, dtype: torch.dtype, device) -> torch.Tensor:
+    """Zeros that stay ours to write whatever mode a later caller is in: torch
+    refuses to write to a tensor made under inference_mode outside of it."""
+    with torch.inference_mode(False):
+        return torch.zeros(size, dtype=dtype, device=device)
+
+
 _ws = {}
 _ws_retired = []
 _ws_lock = threading.Lock()
@@ -178,7 +185,7 @@ def workspace(device: torch.device, batch: int, q_heads: int, kv_heads: int, kv_
             if ws is not None:
                 _ws_retired.append(ws)  # a captured graph may still point at it
             size = max(need, 0 if ws is None else ws.numel() * 2)
-            ws = torch.zeros(size, dtype=torch.uint8, device=torch.device("cuda", idx))
+            ws = _kept_zeros(size, torch.uint8, torch.device("cuda", idx))
             _ws[key] = ws
         return ws
 
@@ -198,7 +205,7 @@ def status_word(device: torch.device) -> torch.Tensor:
         with _ws_lock:
             w = _status.get(idx)
             if w is None:
-                w = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+                w = _kept_zeros(1, torch.int32, torch.device("cuda", idx))
                 torch.cuda.synchronize(idx)  # once: visible to every stream
                 _status[idx] = w
     return w

@@ -307,6 +307,40 @@ def test_the_cache_reports_what_a_step_could_not_append(dev):
     assert int(mine) == N.FK_STATUS_BAD_POSITION and fk.read_status() == 0
 
 
+def test_kept_words_can_be_written_in_any_mode():
+    from fasterkernels_b200 import _native as N
+    with torch.inference_mode():
+        w = N._kept_zeros(3, torch.int32, "cpu")
+        w[:1].fill_(1)
+    w[1:2].fill_(2)
+    with torch.inference_mode():
+        w[2:].fill_(3)
+    assert w.tolist() == [1, 2, 3] and not w.is_inference()
+
+
+@gpu
+def test_read_status_after_first_calls_under_inference_mode(dev):
+    """The status word and the decode workspace are made by whoever calls first."""
+    from fasterkernels_b200 import _native as N
+    kept = dict(N._status), dict(N._ws)
+    N._status.clear()
+    N._ws.clear()
+    try:
+        with torch.inference_mode():
+            q, kp = torch.randn(2, 4, 128, device=dev).half(), torch.randn(4, 2, 16, 128, device=dev).half()
+            bt = torch.tensor([[1], [-1]], dtype=torch.int32, device=dev)
+            lens = torch.tensor([5, 5], dtype=torch.int32, device=dev)
+            fk.paged_flash_decode(q, kp, kp, bt, lens, 16)
+            fk.paged_flash_decode_shared_prefix(q, kp, kp, bt[0], 16, bt, lens, 16)
+        assert fk.read_status() == N.FK_STATUS_BAD_PAGE and fk.read_status() == 0
+        with torch.inference_mode():
+            fk.paged_flash_decode_shared_prefix(q, kp, kp, bt[0], 16, bt, lens, 16)
+            assert fk.read_status() == N.FK_STATUS_BAD_PAGE and fk.read_status() == 0
+    finally:
+        for d, k in zip((N._status, N._ws), kept):
+            d.update(k)
+
+
 @gpu
 def test_the_first_append_of_a_cache_can_be_a_captured_one(dev):
     from fasterkernels_b200 import _native as N
