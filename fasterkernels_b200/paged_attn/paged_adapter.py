@@ -84,7 +84,10 @@ def custom_paged_attention_forward(module, query_states, key_states, value_state
         if layer == 0 or _BOUND.lens is None:
             _BOUND.bt, _, _BOUND.lens = cache.begin_step(_BOUND.seq_ids)
             pages = cache.shared_prefix_pages(_BOUND.seq_ids)
-            _BOUND.shared = pages if shared_prefix_pays(bsz, pages * PAGE_SIZE) else 0
+            own = sum(cache.seq_len(s) for s in _BOUND.seq_ids) / bsz + 1 - pages * PAGE_SIZE
+            pays = shared_prefix_pays(bsz, pages * PAGE_SIZE, own, q_heads=q_heads, kv_heads=cache.num_kv_heads,
+                                      head_dim=head_dim, kv_dtype=cache.dtype)
+            _BOUND.shared = pages if pays else 0
             _BOUND.own = _BOUND.lens - PAGE_SIZE * _BOUND.shared if _BOUND.shared else None
         cache.append_kv_batch(layer, key_states[:, :, -1], value_states[:, :, -1])
         e4m3 = cache.dtype == torch.float8_e4m3fn

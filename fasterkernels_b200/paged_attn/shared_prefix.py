@@ -17,16 +17,59 @@ from ..gqa_decode import HEAD_DIMS, _check_idx, _check_sink
 from ..gqa_decode_hf import _scale_ptr
 
 
-def shared_prefix_pays(batch: int, prefix_len: int) -> bool:
+def _estimates(batch, prefix_len, own_len, q_heads, kv_heads, head_dim, e4m3):
+    """(us of ``paged_flash_decode`` over the whole tables, us with the prefix
+    shared), from what each spends its time on; the factors are fitted to the
+    1170 sizes of ``shared_prefix_pays``.
+
+    Whole tables: a launch, every sequence's elements, and the merge of an item's
+    segments, short and many where sequences are few.  Items of four heads, and
+    of query chunks, start at more.  Shared: three launches (the own part's is
+    longer where tails fill a page at most, four of which go to one CTA); the own
+    elements; an SM's share of the prefix in tiles, which starts late where the
+    own part is on every SM; the join of a row's records."""
+    sms = 148
+    group = max(q_heads // kv_heads, 1)
+    chunks = -(-group // 8)
+    quads = e4m3 and kv_heads % 4 == 0 and 4 < group <= 8
+    items = kv_heads * (chunks + 1) // 2 if chunks > 1 else kv_heads // (4 if quads else 1 + (kv_heads % 2 == 0))
+    elements = 2e-6 * batch * kv_heads * head_dim  # one token of every sequence, in millions
+    segments = min(2 * sms / (batch * items), (prefix_len + own_len) / 64)
+    whole = ((25.5 if quads else 20.5 if chunks > 1 else 11.5 if head_dim > 64 else 10.5)
+             + (0.2 if head_dim > 64 else 0.28) * elements * (prefix_len + own_len)
+             + (0.5 if quads else 0.15 if e4m3 else 0.08) * segments)
+    tiles, row_tiles = -(-prefix_len // 128), -(-batch * group // 128)
+    pairs, odd = divmod(row_tiles, 2)
+    granules = kv_heads * (pairs * tiles + odd * ((tiles + 1) // 2))
+    share = -(-granules // sms)
+    records = min(granules, sms) / (kv_heads * (pairs + odd)) * (2 if row_tiles == 1 else 1)
+    busy = min(1.0, batch * items * ((own_len + 15) // 16) / (4 * sms))
+    shared = (9.5 + (3 if chunks > 1 else 0) + (0 if own_len > 16 else 8.5 if chunks > 1 else 1.8)
+              + 0.34 * elements * own_len + busy * (1.9 + 3.75 * min(share, 4))
+              + (5 if e4m3 else 2.75) * share + 0.11 * records)
+    return whole, shared
+
+
+def shared_prefix_pays(batch: int, prefix_len: int, own_len: int = 64, *, q_heads: int = 32, kv_heads: int = 8,
+                       head_dim: int = 128, kv_dtype=torch.float16) -> bool:
     """Whether reading a prefix once for the batch beats ``paged_flash_decode``
-    over the whole tables, which reads it per sequence.  Device times with 8 KV
-    heads, head dim 128, tails of 64, pools within L2, whole tables against shared
-    prefix: 16-bit pools, 32 query heads, 2 x 2048 tokens 14.8 / 14.0 us, 2 x 4096
-    17.2 / 16.0, 16 x 2048 26.3 / 16.4, 32 x 16384 266 / 40; e4m3 pools 2 x 4096
-    18.8 / 17.0, 16 x 2048 22.5 / 17.4, 32 x 16384 168 / 41 (2 x 16384 loses: 26.6
-    / 28.6); head dim 64, 2 x 4096 14.4 / 14.9, 8 x 2048 15.4 / 13.4.  A call takes
-    19 us on the host, one of ``paged_flash_decode`` 24."""
-    return batch >= 2 and (batch - 1) * prefix_len >= 4096
+    over the whole tables, which reads it per sequence: ``own_len`` tokens of its
+    own a sequence (the mean), heads and pools as given.
+
+    Both were measured on the device at 1170 sizes: 1 to 8 KV heads, groups of 1
+    to 16, head dims 64 and 128, f16 and e4m3 pools, 2 to 128 sequences, prefixes
+    of 128 to 65536 tokens, tails up to 2000, pools past L2 where they can be.  At
+    400 others (drawn of the same ranges) the rule takes a way that is over 10 %
+    slower 21 times, 1.3 % on average; 4096 prefix tokens saved as the rule: 84
+    times, 5.2 %.  In us, whole tables / shared, tails of 64: 8 KV heads, 32 query
+    heads, f16: 2 x 1024 tokens 13.8 / 13.6, 2 x 16384 31.6 / 26.8, 16 x 2048 27.4 /
+    16.7, 64 x 16384 523 / 48; e4m3 2 x 16384 28.2 / 30.5; head dim 64 2 x 4096 15.2 /
+    15.9.  One KV head, 8 query heads: 4 x 16384 21.4 / 25.9.  Tails of 1000 want a
+    longer prefix: 8 KV heads, f16, 4 x 4096 22.5 / 32.0, 16 x 4096 49.6 / 39.4."""
+    if batch < 2 or prefix_len <= 0:
+        return False
+    whole, shared = _estimates(batch, prefix_len, own_len, q_heads, kv_heads, head_dim, kv_dtype == torch.float8_e4m3fn)
+    return shared < whole
 
 
 def paged_flash_decode_shared_prefix(q, k_pool, v_pool, prefix_table, prefix_len, block_table, seq_lens, page_size, *,

@@ -104,6 +104,17 @@ def test_shared_prefix_of_unrelated_single_and_repeated_sequences():
     assert not shared_prefix_pays(1, 10 ** 6) and not shared_prefix_pays(2, 0) and shared_prefix_pays(64, 32768)
 
 
+@pytest.mark.parametrize("batch,prefix,own,kw,pays", [
+    (2, 2048, 64, dict(), True), (16, 2048, 64, dict(), True), (64, 16384, 64, dict(), True), (2, 256, 64, dict(), False),
+    (2, 16384, 64, dict(kv_dtype=E4M3), False), (2, 4096, 64, dict(head_dim=64), False), (16, 4096, 64, dict(head_dim=64), True),
+    (4, 16384, 64, dict(q_heads=8, kv_heads=1), False), (64, 16384, 64, dict(q_heads=8, kv_heads=1), True),
+    (4, 4096, 1000, dict(), False), (16, 4096, 1000, dict(), True), (2, 16384, 1000, dict(), False),
+    (2, 2048, 64, dict(q_heads=64, kv_dtype=E4M3), True), (2, 2048, 64, dict(q_heads=128), True)])
+def test_the_shared_path_is_taken_where_it_measured_faster(batch, prefix, own, kw, pays):
+    """Sizes at which the two ways are 3 % or more apart, in times measured."""
+    assert shared_prefix_pays(batch, prefix, own, **kw) == pays
+
+
 def test_begin_chunk_places_ragged_tokens_and_commits_their_counts():
     c = make()
     a, b, d = (c.allocate_sequence() for _ in range(3))
@@ -452,6 +463,36 @@ def test_paged_adapter_with_queries_that_require_grad(dev, forked):
         assert [c.seq_len(s) for s in ids] == [4417] * len(ids)
     for x, y in zip(*outs):
         assert torch.equal(x, y) and not y.requires_grad
+
+
+@gpu
+def test_paged_adapter_leaves_the_shared_path_where_tails_are_long(dev, monkeypatch):
+    """The same forks with short and long own parts: the rule is asked with what is bound."""
+    from fasterkernels_b200.paged_attn import paged_adapter
+    asked = []
+    monkeypatch.setattr(paged_adapter, "shared_prefix_pays", lambda *a, **k: asked.append((a, k)) or shared_prefix_pays(*a, **k))
+    taken = []
+    real = paged_adapter.paged_flash_decode_shared_prefix
+    monkeypatch.setattr(paged_adapter, "paged_flash_decode_shared_prefix", lambda *a, **k: taken.append(a[4]) or real(*a, **k))
+    c = make(pages=4 * 120, seqs=5, blocks=140, device=str(dev), layers=1, heads=8)
+    a = c.allocate_sequence()
+    k = torch.randn(8, 1024, 128, device=dev).half()
+    c.write_prefill(a, 0, k, k)
+    ids = [c.fork_sequence(a, 1024) for _ in range(4)]
+    for tail in (20, 980):
+        c.begin_chunk(ids, [tail] * 4)
+        x = torch.randn(4 * tail, 8, 128, device=dev).half()
+        c.append_qkv_batch(0, x, x, x, None, None)
+        c.end_step()
+        fk.set_paged_attention_cache(c, ids)
+        try:
+            q = torch.randn(4, 32, 1, 128, device=dev).half()
+            x = torch.randn(4, 8, 1, 128, device=dev).half()
+            fk.custom_paged_attention_forward(_Module(0), q, x, x, None, 128 ** -0.5)
+        finally:
+            fk.set_paged_attention_cache(None, [])
+    heads = dict(q_heads=32, kv_heads=8, head_dim=128, kv_dtype=torch.float16)
+    assert asked == [((4, 1024, 21), heads), ((4, 1024, 1002), heads)] and taken == [1024]
 
 
 @gpu
