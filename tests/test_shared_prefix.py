@@ -309,6 +309,29 @@ def test_query_types_scales_and_output_types_over_e4m3(dev):
 
 
 @gpu
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("G,KVH", [(5, 4), (6, 8), (7, 4), (8, 4), (8, 8)])
+@pytest.mark.parametrize("qtype", [torch.float16, torch.bfloat16, E4M3])
+def test_own_tokens_of_four_heads_an_item(dev, G, KVH, qtype, aligned):
+    """e4m3 pools, KV heads a multiple of four, groups of 5 to 8: the own part
+    takes four KV heads at a time, with 32 slots a record, where the rows of q are
+    16-byte aligned, and two where they are not."""
+    c = make(dev, 500, [700, 0, 1, 33, 4000], G * KVH, KVH, dtype=torch.bfloat16 if qtype == torch.bfloat16 else torch.float16,
+             pool=E4M3, sinks=True, seed=G + KVH)
+    q, sq = c["q"], None
+    if qtype == E4M3:
+        q, sq = (100 * q).clamp(-448, 448).to(E4M3), torch.tensor(0.01, device=dev)
+    if not aligned:
+        wide = torch.zeros(5, G * KVH, 130 if qtype != E4M3 else 136, dtype=q.dtype, device=dev)
+        wide[..., 2:130].copy_(q)
+        q = wide[..., 2:130]
+    got = fk.paged_flash_decode_shared_prefix(q, c["k"], c["v"], c["table"], c["plen"], c["bt"], c["seq"], 16, s_aux=c["sink"],
+                                              scale_q=sq, scale_k=c["sk"], scale_v=c["sv"])
+    # what the kernel multiplies: q (times its scale) rounded to f16
+    check(c, got, q=(q.float() * sq).half().double() if sq is not None else q.half().double())
+
+
+@gpu
 def test_offsets_past_32_bits(dev):
     P = 140_000  # pages of 16 KB: the last ones start past 2^31 elements
     pages = [P - 1, 131_073, 5, P - 2, 139_000, 131_072]
