@@ -22,7 +22,11 @@
 //   so that it never waits for the chain P V, Q K^T.  (With 128-token items there
 //   is room for one S a stream, and that chain, 1100 cycles, was added to every
 //   tile: 395 us instead of 319, at that time, for the long case below.)  P (f16, or bf16 for bf16 KV)
-//   overwrites half of its own S and is the A operand of O += P V from there.
+//   overwrites half of its own S and is the A operand of O += P V from there:
+//   the type that V has or is widened to, since the tensor cores take A and B of
+//   one 16-bit type (f32 P would be a second product for its low half).  That
+//   rounding is of the size of the output's own, so errors are 1.1 to 1.4 times
+//   those of 32-bit P; the sum of P is of the unrounded ones, in 32 bits.
 //
 // Work is cut like the decode kernel's: units (KV head, one or two row tiles)
 // laid end to end in granules (dual: one token tile, parity: two), each CTA of
@@ -47,10 +51,10 @@
 // cycles: the chain P ready -> P V, Q K^T issue -> S ready passes through one
 // issuing warp, and e4m3 widening takes 512 cycles of shared-memory bandwidth more.
 // Device times, own part and join included (B200): long case, 128 sequences x 64
-// heads (8 KV heads), 65536 tokens of e4m3 + tails up to 1000, 300 us = 0.92
-// PFLOP/s; 64 x 32 heads, 32768 tokens of f16 + tails up to 512, 70 us, of which
+// heads (8 KV heads), 65536 tokens of e4m3 + tails up to 1000, 303 us = 0.92
+// PFLOP/s; 64 x 32 heads, 32768 tokens of f16 + tails up to 512, 71 us, of which
 // the own part's reads take 20 to 27 and the join 9; 2 x 32 heads, 131072 tokens of
-// bf16, 106 us = 5.1 TB/s; 4 x 32 heads, 1000 tokens, 16 us, three kernels'
+// bf16, 108 us = 5.0 TB/s; 4 x 32 heads, 1000 tokens, 17 us, three kernels'
 // latencies.
 #include <cuda_fp8.h>
 
